@@ -1,0 +1,299 @@
+// paged_rope.cu — head RMSNorm, rotary positions and the append of new tokens
+// to a paged cache (include/m27b_paged.h), in one pass over the projections.
+//
+//   x' = x * rsqrt(mean(x^2) + eps) * w                      (where w is given)
+//   (u, v) -> (u c - v s, u s + v c) for each of the first n_rot / 2 pairs of
+//   the head, (c, s) = the position's table entry; q to q_out, k to its slot
+//   of the cache, v to its slot as it is; one rounding to 16 bits at the end.
+//
+// A warp takes one head of one token: lane l holds its values [l V, l V + V),
+// V = head_dim / 32, so the mean is one butterfly, and the second value of a
+// half-layout pair lies n_rot / 2 values, a whole number of lanes, away.
+// Bounded by the bytes: each projection value is read once and written once
+// in 16 bits; the table (256 bytes a token at n_rot = 64) stays in L2.
+#include "paged_common.cuh"
+
+namespace m27b {
+
+struct RopeArgs {
+    M27BPagedKV kv;
+    M27BPagedBatch bt;
+    M27BRope rope;
+    M27BHeads h;
+    void *q_out;
+    long long q_out_stride;
+    int *status;
+};
+
+// Sequence of token t: the number of ends cu_q[1..n] at or before t (n: none).
+// 32 probes a step.
+M27B_DI int find_seq(const int *cu_q, int n, int t, int lane) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int step = (hi - lo + 31) / 32, i = lo + lane * step + step - 1;
+        const bool past = i < hi && __ldg(cu_q + i + 1) <= t;
+        lo += __popc(__ballot_sync(0xffffffffu, past)) * step;
+        if (step == 1) break;
+        hi = min(hi, lo + step - 1);
+    }
+    return min(lo, n);
+}
+
+template <bool F32, bool BF, int V>
+M27B_DI void load_head(const void *base, long long off, float (&x)[V]) {
+    if constexpr (F32) {
+        const float *p = (const float *)base + off;
+        if constexpr (V == 2) {
+            const float2 t = __ldcs((const float2 *)p);
+            x[0] = t.x, x[1] = t.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < V / 4; ++c) {
+                const float4 t = __ldcs((const float4 *)p + c);
+                x[4 * c] = t.x, x[4 * c + 1] = t.y, x[4 * c + 2] = t.z, x[4 * c + 3] = t.w;
+            }
+        }
+    } else {
+        const uint16_t *p = (const uint16_t *)base + off;
+        uint32_t w[V / 2];
+        if constexpr (V == 2) w[0] = __ldcs((const unsigned *)p);
+        else if constexpr (V == 4) {
+            const uint2 t = __ldcs((const uint2 *)p);
+            w[0] = t.x, w[1] = t.y;
+        } else {
+            const uint4 t = __ldcs((const uint4 *)p);
+            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+        }
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = Half16<BF>::up(w[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+}
+
+template <bool BF, int V>
+M27B_DI void store_head(void *base, long long off, const float (&x)[V]) {
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = Half16<BF>::down(x[2 * i], x[2 * i + 1]);
+    uint16_t *p = (uint16_t *)base + off;
+    if constexpr (V == 2) *(unsigned *)p = w[0];
+    else if constexpr (V == 4) *(uint2 *)p = make_uint2(w[0], w[1]);
+    else *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool F32, bool BF, int V>
+__global__ void __launch_bounds__(256) k_rope_append(const RopeArgs a) {
+    constexpr int HD = 32 * V;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int n_rows = a.h.n_q + 2 * a.kv.n_kv;
+    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long long t64 = w / n_rows;
+    if (t64 >= a.bt.n_tok) return;
+    const int t = (int)t64, r = (int)(w - t64 * n_rows);
+    const int b = find_seq(a.bt.cu_q, a.bt.n_seq, t, lane);
+    if (b >= a.bt.n_seq || t < __ldg(a.bt.cu_q + b)) return;
+    const int row = seq_row(a.bt, b, a.kv.n_rows);
+    const int p = row < 0 ? -1 : __ldg(a.bt.lens + row) - __ldg(a.bt.cu_q + b + 1) + t;
+    const int rp = a.rope.positions ? __ldg(a.rope.positions + t) : p;
+    const int pc = p / a.kv.page_size;
+    const int page = p >= 0 && pc < a.kv.n_cols ? __ldg(a.kv.table + (long long)row * a.kv.n_cols + pc) : -1;
+    if (page < 0 || page >= a.kv.n_pages || rp < 0 || rp >= a.rope.n_pos) {
+        if (lane == 0) paged_bad(a.status);
+        return;
+    }
+    const long long slot = page * a.kv.page_stride + (long long)(p - pc * a.kv.page_size) * a.kv.n_kv * HD;
+    float x[V];
+    if (r >= a.h.n_q + a.kv.n_kv) {
+        const int j = r - a.h.n_q - a.kv.n_kv;
+        load_head<F32, BF>(a.h.v, t * a.h.v_stride + j * HD + lane * V, x);
+        store_head<BF>(a.kv.v, slot + j * HD + lane * V, x);
+        return;
+    }
+    const bool is_q = r < a.h.n_q;
+    const int j = is_q ? r : r - a.h.n_q;
+    load_head<F32, BF>(is_q ? a.h.q : a.h.k, t * (is_q ? a.h.q_stride : a.h.k_stride) + j * HD + lane * V, x);
+    const float *nw = is_q ? a.h.q_norm : a.h.k_norm;
+    if (nw) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss = fmaf(x[i], x[i], ss);
+        const float sc = 1.0f / sqrtf(warp_sum(ss) / (float)HD + a.h.eps);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = x[i] * sc * __ldg(nw + lane * V + i);
+    }
+    const int d0 = lane * V, half = a.rope.n_rot / 2;
+    const float2 *tab = (const float2 *)a.rope.table + (long long)rp * half;
+    if (a.rope.interleaved) {
+        if (d0 < a.rope.n_rot)
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 cs = __ldg(tab + d0 / 2 + i);
+                const float u = x[2 * i], v = x[2 * i + 1];
+                x[2 * i] = u * cs.x - v * cs.y;
+                x[2 * i + 1] = u * cs.y + v * cs.x;
+            }
+    } else {
+        const int dl = half / V;  // lanes between the two values of a pair
+        const bool first = d0 < half;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], first ? lane + dl : lane - dl);
+        if (d0 < a.rope.n_rot)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float2 cs = __ldg(tab + (first ? d0 : d0 - half) + i);
+                x[i] = first ? x[i] * cs.x - o[i] * cs.y : o[i] * cs.y + x[i] * cs.x;
+            }
+    }
+    if (is_q) store_head<BF>(a.q_out, t * a.q_out_stride + j * HD + d0, x);
+    else store_head<BF>(a.kv.k, slot + j * HD + d0, x);
+}
+
+template <bool F32, bool BF>
+cudaError_t rope_launch(const RopeArgs &a, cudaStream_t st) {
+    const long long warps = (long long)a.bt.n_tok * (a.h.n_q + 2 * a.kv.n_kv);
+    const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
+    switch (a.kv.head_dim) {
+    case 64: return launch_pdl(k_rope_append<F32, BF, 2>, grid, block, 0, st, a);
+    case 128: return launch_pdl(k_rope_append<F32, BF, 4>, grid, block, 0, st, a);
+    default: return launch_pdl(k_rope_append<F32, BF, 8>, grid, block, 0, st, a);
+    }
+}
+
+struct RopeTable {
+    float2 *out;
+    int n_pos, half;
+    double theta;
+    M27BRopeScaling s;
+    double lo, hi, mul;
+};
+
+// One thread per (position, pair); the frequency and the angle in fp64, since
+// an fp32 angle is off by up to 2^-24 of its size: 0.06 at a position of 10^6.
+__global__ void __launch_bounds__(256) k_rope_table(const RopeTable a) {
+    const long long n = (long long)a.n_pos * a.half;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        const long long p = i / a.half;
+        const int j = (int)(i - p * a.half);
+        double f = pow(a.theta, -(double)j / a.half);
+        if (a.s.kind == M27B_ROPE_LINEAR) f /= a.s.factor;
+        if (a.s.kind == M27B_ROPE_YARN) {
+            const double r = fmin(fmax((j - a.lo) / fmax(a.hi - a.lo, 0.001), 0.0), 1.0);
+            f = f / a.s.factor * r + f * (1.0 - r);
+        }
+        double s, c;
+        sincos((double)p * f, &s, &c);
+        a.out[i] = make_float2((float)(c * a.mul), (float)(s * a.mul));
+    }
+}
+
+bool paged_check_kv(const M27BPagedKV *kv, const char *what, char *err, size_t cap) {
+    if (!kv) return paged_fail(err, cap, "%s: null cache", what);
+    if (!kv->k || !kv->v || !kv->table) return paged_fail(err, cap, "%s: null pool or table", what);
+    if (((uintptr_t)kv->k | (uintptr_t)kv->v) & 15u)
+        return paged_fail(err, cap, "%s: pools must be 16-byte aligned", what);
+    if (kv->type != M27B_TYPE_F16 && kv->type != M27B_TYPE_BF16)
+        return paged_fail(err, cap, "%s: the cache's type must be f16 or bf16 (got %u)", what, kv->type);
+    if (kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)))
+        return paged_fail(err, cap, "%s: page_size must be 16, 32, 64, 128 or 256 (got %d)", what, kv->page_size);
+    if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+        return paged_fail(err, cap, "%s: head_dim must be 64, 128 or 256 (got %d)", what, kv->head_dim);
+    if (kv->n_kv < 1 || kv->n_kv > 1024) return paged_fail(err, cap, "%s: bad n_kv (%d)", what, kv->n_kv);
+    if (kv->n_pages < 1 || kv->n_rows < 1 || kv->n_cols < 1)
+        return paged_fail(err, cap, "%s: empty cache (%d pages, %d rows of %d)", what, kv->n_pages, kv->n_rows, kv->n_cols);
+    if ((long long)kv->n_cols * kv->page_size > 0x7fffffffll)
+        return paged_fail(err, cap, "%s: n_cols x page_size passes 31 bits", what);
+    if (kv->page_stride < (long long)kv->page_size * kv->n_kv * kv->head_dim || kv->page_stride % 8)
+        return paged_fail(err, cap, "%s: page_stride (%lld) must be a multiple of 8, at least a page", what, kv->page_stride);
+    if (kv->page_stride > (1ll << 62) / 2 / kv->n_pages)
+        return paged_fail(err, cap, "%s: page_stride (%lld) too large", what, kv->page_stride);
+    return true;
+}
+
+bool paged_check_batch(const M27BPagedBatch *b, const M27BPagedKV *kv, const char *what, char *err, size_t cap) {
+    if (!b || !b->cu_q || !b->lens) return paged_fail(err, cap, "%s: null batch, cu_q or lens", what);
+    if (b->n_seq < 0 || b->n_tok < 0) return paged_fail(err, cap, "%s: bad n_seq (%d) or n_tok (%d)", what, b->n_seq, b->n_tok);
+    if (!b->rows && b->n_seq > kv->n_rows)
+        return paged_fail(err, cap, "%s: %d sequences and %d table rows", what, b->n_seq, kv->n_rows);
+    return true;
+}
+
+}  // namespace m27b
+
+using namespace m27b;
+
+extern "C" {
+
+bool m27b_rope_table(float *table, int n_pos, int n_rot, double theta, const M27BRopeScaling *scaling,
+                     cudaStream_t stream, char *err, size_t err_cap) {
+    const char *what = "m27b_rope_table";
+    if (!table || ((uintptr_t)table & 7u)) return paged_fail(err, err_cap, "%s: table must be 8-byte aligned", what);
+    if (n_pos < 1) return paged_fail(err, err_cap, "%s: n_pos must be positive (got %d)", what, n_pos);
+    if (n_rot < 2 || n_rot % 2 || n_rot > 65536) return paged_fail(err, err_cap, "%s: n_rot must be even (got %d)", what, n_rot);
+    if (!(theta > 0.0)) return paged_fail(err, err_cap, "%s: theta must be positive", what);
+    RopeTable a = {};
+    a.out = (float2 *)table, a.n_pos = n_pos, a.half = n_rot / 2, a.theta = theta, a.mul = 1.0;
+    if (scaling) a.s = *scaling;
+    if (a.s.kind < M27B_ROPE_NONE || a.s.kind > M27B_ROPE_YARN)
+        return paged_fail(err, err_cap, "%s: unknown scaling %d", what, a.s.kind);
+    if (a.s.kind != M27B_ROPE_NONE && !(a.s.factor >= 1.0f))
+        return paged_fail(err, err_cap, "%s: the scaling factor must be at least 1", what);
+    if (a.s.kind == M27B_ROPE_YARN) {
+        if (a.s.original_ctx < 1 || !(a.s.beta_fast > 0.0f) || !(a.s.beta_slow > 0.0f) || theta == 1.0)
+            return paged_fail(err, err_cap, "%s: yarn needs original_ctx, beta_fast and beta_slow", what);
+        // pair that turns `beta` times over the original context
+        auto pair = [&](double beta) {
+            return n_rot * log(a.s.original_ctx / (2.0 * 3.14159265358979323846 * beta)) / (2.0 * log(theta));
+        };
+        a.lo = fmax(0.0, floor(pair(a.s.beta_fast)));
+        a.hi = fmin((double)n_rot - 1.0, ceil(pair(a.s.beta_slow)));
+        a.mul = a.s.attn_factor > 0.0f ? (double)a.s.attn_factor : 0.1 * log((double)a.s.factor) + 1.0;
+    }
+    const long long n = (long long)n_pos * a.half;
+    const unsigned grid = (unsigned)((n + 255) / 256 < 16384 ? (n + 255) / 256 : 16384);
+    k_rope_table<<<grid, 256, 0, stream>>>(a);
+    return paged_ok(cudaGetLastError(), what, err, err_cap);
+}
+
+bool m27b_rope_append(const M27BPagedKV *kv, const M27BPagedBatch *batch, const M27BRope *rope, const M27BHeads *heads,
+                      void *q_out, long long q_out_stride, cudaStream_t stream, char *err, size_t err_cap) {
+    const char *what = "m27b_rope_append";
+    if (!paged_check_kv(kv, what, err, err_cap) || !paged_check_batch(batch, kv, what, err, err_cap)) return false;
+    if (!rope || !rope->table || ((uintptr_t)rope->table & 15u))
+        return paged_fail(err, err_cap, "%s: the rope table must be 16-byte aligned", what);
+    if (rope->n_pos < 1 || rope->n_rot < 16 || rope->n_rot % 16 || rope->n_rot > kv->head_dim)
+        return paged_fail(err, err_cap, "%s: n_rot must be a multiple of 16, at most head_dim (got %d)", what, rope->n_rot);
+    if (!batch->n_seq || !batch->n_tok) return paged_ok(cudaSuccess, what, err, err_cap);
+    if (!heads || !heads->k || !heads->v) return paged_fail(err, err_cap, "%s: null k or v", what);
+    if (heads->n_q < 0 || heads->n_q > 65536) return paged_fail(err, err_cap, "%s: bad n_q (%d)", what, heads->n_q);
+    if (heads->n_q && (!heads->q || !q_out)) return paged_fail(err, err_cap, "%s: null q or q_out", what);
+    const bool f32 = heads->src_type == M27B_TYPE_F32;
+    if (!f32 && heads->src_type != kv->type)
+        return paged_fail(err, err_cap, "%s: q, k, v must be f32 or of the cache's type (got %u)", what, heads->src_type);
+    const int per16 = f32 ? 4 : 8;
+    if (((uintptr_t)heads->q | (uintptr_t)heads->k | (uintptr_t)heads->v | (uintptr_t)q_out | (uintptr_t)heads->q_norm |
+         (uintptr_t)heads->k_norm) & 15u)
+        return paged_fail(err, err_cap, "%s: q, k, v, q_out and norm weights must be 16-byte aligned", what);
+    if (heads->q_stride % per16 || heads->k_stride % per16 || heads->v_stride % per16 || q_out_stride % 8)
+        return paged_fail(err, err_cap, "%s: strides must be multiples of 16 bytes", what);
+    const long long hd = kv->head_dim;
+    if (heads->k_stride < kv->n_kv * hd || heads->v_stride < kv->n_kv * hd ||
+        (heads->n_q && (heads->q_stride < heads->n_q * hd || q_out_stride < heads->n_q * hd)))
+        return paged_fail(err, err_cap, "%s: a token's stride is shorter than its heads", what);
+    const void *q = heads->q;
+    if (heads->n_q && q_out == q && (f32 || q_out_stride != heads->q_stride))
+        return paged_fail(err, err_cap, "%s: q_out may be q only with its type and stride", what);
+    if ((long long)batch->n_tok * (heads->n_q + 2 * kv->n_kv) > 0x7fffffffll * 8)
+        return paged_fail(err, err_cap, "%s: too many heads", what);
+    RopeArgs a = {*kv, *batch, *rope, *heads, q_out, q_out_stride, status_ptr_current()};
+    const bool bf = kv->type == M27B_TYPE_BF16;
+    cudaError_t e = f32 ? (bf ? rope_launch<true, true>(a, stream) : rope_launch<true, false>(a, stream))
+                        : (bf ? rope_launch<false, true>(a, stream) : rope_launch<false, false>(a, stream));
+    return paged_ok(e, what, err, err_cap);
+}
+
+}  // extern "C"

@@ -762,3 +762,314 @@ def speculative_generate(target, draft, prompt, n_new, k=7):
 
 
 M27B_VERIFY_MAX = 16
+
+# --------------------------------------------------------------------------
+# paged key/value cache (include/m27b_paged.h)
+
+BF16 = 30
+ROPE_NONE, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
+PAGES_FULL, PAGES_BAD = 1, 2
+
+
+class _PagedKV(ctypes.Structure):
+    """M27BPagedKV"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p), ("type", ctypes.c_uint32),
+                ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int), ("n_kv", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("n_rows", ctypes.c_int), ("n_cols", ctypes.c_int),
+                ("page_stride", ctypes.c_longlong)]
+
+
+class _PagedBatch(ctypes.Structure):
+    """M27BPagedBatch"""
+    _fields_ = [("cu_q", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("rows", ctypes.c_void_p),
+                ("n_seq", ctypes.c_int), ("n_tok", ctypes.c_int)]
+
+
+class _RopeScaling(ctypes.Structure):
+    """M27BRopeScaling"""
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_float), ("original_ctx", ctypes.c_int),
+                ("beta_fast", ctypes.c_float), ("beta_slow", ctypes.c_float), ("attn_factor", ctypes.c_float)]
+
+
+class _Rope(ctypes.Structure):
+    """M27BRope"""
+    _fields_ = [("table", ctypes.c_void_p), ("n_pos", ctypes.c_int), ("n_rot", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("positions", ctypes.c_void_p)]
+
+
+class _Heads(ctypes.Structure):
+    """M27BHeads"""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_longlong),
+                ("k_stride", ctypes.c_longlong), ("v_stride", ctypes.c_longlong), ("src_type", ctypes.c_uint32),
+                ("n_q", ctypes.c_int), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
+class _Pages(ctypes.Structure):
+    """M27BPages"""
+    _fields_ = [("ref", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int), ("n_rows", ctypes.c_int),
+                ("n_cols", ctypes.c_int)]
+
+
+class _PagePool(ctypes.Structure):
+    """M27BPagePool"""
+    _fields_ = [("base", ctypes.c_void_p), ("n_planes", ctypes.c_int), ("plane_stride", ctypes.c_size_t),
+                ("page_stride", ctypes.c_size_t), ("page_bytes", ctypes.c_size_t)]
+
+
+def _paged_lib():
+    L = lib()
+    if getattr(L, "_paged_sigs", False):
+        return L
+    vp, cp, sz, i32, ll, b = (ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_longlong,
+                              ctypes.c_bool)
+    kv, bt, pg, pool = (ctypes.POINTER(t) for t in (_PagedKV, _PagedBatch, _Pages, _PagePool))
+    sig = {
+        "m27b_rope_table": (b, [vp, i32, i32, ctypes.c_double, ctypes.POINTER(_RopeScaling), vp, cp, sz]),
+        "m27b_rope_append": (b, [kv, bt, ctypes.POINTER(_Rope), ctypes.POINTER(_Heads), vp, ll, vp, cp, sz]),
+        "m27b_paged_attn_scratch_bytes": (sz, [i32, i32, i32]),
+        "m27b_paged_attn": (b, [kv, bt, vp, ll, i32, ctypes.c_float, i32, vp, ll, vp, vp, vp, cp, sz]),
+        "m27b_pages_scratch_bytes": (sz, [i32, i32, i32]),
+        "m27b_pages_resize": (b, [pg, pool, i32, vp, vp, i32, vp, vp, vp, cp, sz]),
+        "m27b_pages_fork": (b, [pg, pool, i32, vp, vp, i32, vp, vp, vp, cp, sz]),
+        "m27b_pages_free": (b, [pg, vp, i32, vp, cp, sz]),
+        "m27b_pages_compact": (b, [pg, pool, i32, vp, vp, vp, cp, sz]),
+        "m27b_pages_copy": (b, [pool, i32, i32, vp, vp, i32, vp, cp, sz]),
+    }
+    for name, (res, args) in sig.items():
+        f = getattr(L, name)
+        f.restype = res
+        f.argtypes = args
+    L._paged_sigs = True
+    return L
+
+
+def _paged_type(dtype):
+    import torch
+    t = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}.get(dtype)
+    if t is None:
+        raise M27BError(f"paged cache: unsupported type {dtype}")
+    return t
+
+
+def _int32(t, what, n=None):
+    """The data pointer of a contiguous device int32 tensor (None passes)."""
+    import torch
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() < n):
+        raise M27BError(f"{what} must be a contiguous int32 device tensor" + (f" of at least {n} values" if n else ""))
+    return t.data_ptr()
+
+
+def _token_heads(t, what, n_tok, n_head, head_dim, dtype):
+    """(pointer, token stride) of [n_tok, n_head, head_dim] rows whose heads are contiguous."""
+    if t.dim() != 3 or t.shape[0] != n_tok or t.shape[1] != n_head or t.shape[2] != head_dim or t.dtype != dtype \
+            or not t.is_cuda:
+        raise M27BError(f"{what} must be a device tensor [{n_tok}, {n_head}, {head_dim}] of {dtype} "
+                        f"(got {list(t.shape)} of {t.dtype})")
+    s = t.stride()
+    if (s[2] != 1 and head_dim > 1) or (s[1] != head_dim and n_head > 1):
+        raise M27BError(f"{what}: a token's heads must be contiguous (strides {s})")
+    return t.data_ptr(), s[0] if n_tok > 1 else n_head * head_dim
+
+
+class PagedKV:
+    """One layer's pools of a paged cache, with the page table.
+
+    k, v: device tensors [n_pages, page_size, n_kv, head_dim] in f16 or bf16,
+    contiguous but for the first stride (the pools of several layers may
+    interleave); table: int32 [n_rows, n_cols] page ids."""
+
+    def __init__(self, k, v, table):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise M27BError("PagedKV: k and v must be [n_pages, page_size, n_kv, head_dim] of one type and layout")
+        n_pages, page_size, n_kv, head_dim = k.shape
+        s = k.stride()
+        want = (n_kv * head_dim, head_dim, 1)
+        if any(n > 1 and a != b for n, a, b in zip(k.shape[1:], s[1:], want)) or not k.is_cuda or not v.is_cuda:
+            raise M27BError(f"PagedKV: a page must be contiguous on the device (strides {s})")
+        if table.dim() != 2:
+            raise M27BError("PagedKV: table must be [n_rows, n_cols]")
+        self.k, self.v, self.table = k, v, table
+        self.n_kv, self.head_dim, self.dtype = n_kv, head_dim, k.dtype
+        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _int32(table, "table"), _paged_type(k.dtype), n_pages, page_size,
+                          n_kv, head_dim, table.shape[0], table.shape[1],
+                          s[0] if n_pages > 1 else page_size * n_kv * head_dim)
+        self._ref = ctypes.byref(self.c)
+        _paged_lib()
+
+
+def _batch(kv, cu_q, lens, rows, n_tok):
+    n_seq = cu_q.numel() - 1
+    if n_seq < 0:
+        raise M27BError("cu_q needs n_seq + 1 values")
+    return _PagedBatch(_int32(cu_q, "cu_q"), _int32(lens, "lens", kv.c.n_rows if rows is not None else n_seq),
+                       _int32(rows, "rows", n_seq), n_seq, n_tok)
+
+
+def rope_table(n_pos, n_rot, theta, kind=ROPE_NONE, factor=1.0, original_ctx=0, beta_fast=32.0, beta_slow=1.0,
+               attn_factor=0.0, device="cuda", stream=None):
+    """cos / sin of every position's rotary angles, fp32 [n_pos, n_rot / 2, 2] (m27b_rope_table)."""
+    import torch
+    if n_pos < 1 or n_rot < 2 or n_rot % 2:
+        raise M27BError(f"rope_table: bad n_pos ({n_pos}) or n_rot ({n_rot})")
+    out = torch.empty(n_pos, n_rot // 2, 2, dtype=torch.float32, device=device)
+    s = _RopeScaling(kind, factor, original_ctx, beta_fast, beta_slow, attn_factor)
+    err = ctypes.create_string_buffer(ERR_CAP)
+    _check(_paged_lib().m27b_rope_table(_ptr(out), n_pos, n_rot, theta, ctypes.byref(s), _stream(stream), err, ERR_CAP),
+           err, "m27b_rope_table")
+    return out
+
+
+def rope_append(kv, q, k, v, cu_q, lens, rope, q_out, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, rows=None,
+                positions=None, stream=None):
+    """Head RMSNorm and rotary positions of the new tokens' q [n_tok, n_q, hd]
+    and k [n_tok, n_kv, hd]; q goes to q_out, k and v to the tokens' slots of
+    the cache (m27b_rope_append).  cu_q [n_seq + 1]: each sequence's token
+    rows; lens: positions of each table row, the new ones included; rope: a
+    table of rope_table.  q may be None (append only)."""
+    import torch
+    n_tok, n_q = k.shape[0], 0 if q is None else q.shape[1]
+    kp, ks = _token_heads(k, "k", n_tok, kv.n_kv, kv.head_dim, k.dtype)
+    vp, vs = _token_heads(v, "v", n_tok, kv.n_kv, kv.head_dim, k.dtype)
+    qp, qs, op, os_ = None, 0, None, 0
+    if q is not None:
+        qp, qs = _token_heads(q, "q", n_tok, n_q, kv.head_dim, k.dtype)
+        op, os_ = _token_heads(q_out, "q_out", n_tok, n_q, kv.head_dim, kv.dtype)
+    if rope.dim() != 3 or rope.shape[2] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
+        raise M27BError("rope must be an fp32 table [n_pos, n_rot / 2, 2]")
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != kv.head_dim or not w.is_contiguous()):
+            raise M27BError(f"{name} must be {kv.head_dim} fp32 values")
+    bt = _batch(kv, cu_q, lens, rows, n_tok)
+    rp = _Rope(rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], 1 if interleaved else 0,
+               _int32(positions, "positions", n_tok))
+    hd = _Heads(qp, kp, vp, qs, ks, vs, _paged_type(k.dtype), n_q, q_norm.data_ptr() if q_norm is not None else None,
+                k_norm.data_ptr() if k_norm is not None else None, eps)
+    err = ctypes.create_string_buffer(ERR_CAP)
+    _check(_paged_lib().m27b_rope_append(kv._ref, ctypes.byref(bt), ctypes.byref(rp), ctypes.byref(hd), op, os_,
+                                         _stream(stream), err, ERR_CAP), err, "m27b_rope_append")
+    return q_out
+
+
+def paged_attn_scratch(n_q, n_kv, head_dim, device="cuda"):
+    """Scratch of paged_attn (zeroed; one for each stream that calls it)."""
+    import torch
+    n = _paged_lib().m27b_paged_attn_scratch_bytes(n_q, n_kv, head_dim)
+    if n == 0:
+        raise M27BError(f"paged_attn: unsupported heads ({n_q} on {n_kv}, head_dim {head_dim})")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_attn(kv, q, cu_q, lens, out, scratch, scale=None, window=0, lse=None, rows=None, stream=None):
+    """Causal attention of the new tokens q [n_tok, n_q, hd] over the cache
+    (m27b_paged_attn): one token or many per sequence, the newest at position
+    lens - 1; window > 0 limits a token to the last `window` positions; lse
+    [n_tok, n_q] fp32 receives the log sum of exponentials.  scale defaults to
+    1 / sqrt(hd)."""
+    import torch
+    n_tok, n_q = q.shape[0], q.shape[1]
+    qp, qs = _token_heads(q, "q", n_tok, n_q, kv.head_dim, kv.dtype)
+    op, os_ = _token_heads(out, "out", n_tok, n_q, kv.head_dim, kv.dtype)
+    L = _paged_lib()
+    if scratch.numel() * scratch.element_size() < L.m27b_paged_attn_scratch_bytes(n_q, kv.n_kv, kv.head_dim):
+        raise M27BError("paged_attn: scratch is too small for these heads")
+    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n_tok * n_q or not lse.is_contiguous()):
+        raise M27BError(f"lse must be {n_tok} x {n_q} fp32 values")
+    bt = _batch(kv, cu_q, lens, rows, n_tok)
+    err = ctypes.create_string_buffer(ERR_CAP)
+    _check(L.m27b_paged_attn(kv._ref, ctypes.byref(bt), qp, qs, n_q, kv.head_dim ** -0.5 if scale is None else scale,
+                             window, op, os_, lse.data_ptr() if lse is not None else None, scratch.data_ptr(),
+                             _stream(stream), err, ERR_CAP), err, "m27b_paged_attn")
+    return out
+
+
+class PageSet:
+    """The pages of a paged cache: which rows of `table` hold which pages, how
+    many hold each (`ref`, int32 [n_pages]; free where it is 0) and the rows'
+    lengths (`lens`, int32 [n_rows]).
+
+    pool: the data, a device tensor (or up to two, one for keys and one for
+    values) [n_planes, n_pages, ...] whose pages are contiguous; a plane is a
+    layer's keys or values.  Requests are device int32 tensors.  A refused
+    request (too few free pages, or a bad one) changes nothing and shows in
+    check()."""
+
+    def __init__(self, table, ref, lens, page_size, pool, max_requests=None):
+        import torch
+        if table.dim() != 2 or lens.numel() != table.shape[0]:
+            raise M27BError("PageSet: table must be [n_rows, n_cols], lens [n_rows]")
+        self.table, self.ref, self.lens, self.page_size = table, ref, lens, page_size
+        self.pools = list(pool) if isinstance(pool, (list, tuple)) else [pool]
+        n_pages = ref.numel()
+        arr = []
+        for p in self.pools:
+            if p.dim() < 3 or p.shape[1] != n_pages or not p.is_cuda or not p[0, 0].is_contiguous():
+                raise M27BError(f"PageSet: a pool is [n_planes, {n_pages}, ...] on the device, its pages contiguous")
+            es = p.element_size()
+            page_bytes = p[0, 0].numel() * es
+            arr.append(_PagePool(p.data_ptr(), p.shape[0], p.stride(0) * es if p.shape[0] > 1 else 0,
+                                 p.stride(1) * es if n_pages > 1 else page_bytes, page_bytes))
+        self._pools = (_PagePool * len(arr))(*arr)
+        self.c = _Pages(_int32(ref, "ref"), _int32(table, "table"), _int32(lens, "lens"), n_pages, page_size,
+                        table.shape[0], table.shape[1])
+        self._ref = ctypes.byref(self.c)
+        self.max_requests = table.shape[0] if max_requests is None else max_requests
+        L = _paged_lib()
+        self._scratch = torch.empty(L.m27b_pages_scratch_bytes(n_pages, table.shape[0], self.max_requests),
+                                    dtype=torch.uint8, device=ref.device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=ref.device)
+
+    @classmethod
+    def empty(cls, n_rows, n_cols, n_pages, page_size, pool, device="cuda"):
+        """A cache that holds nothing."""
+        import torch
+        return cls(torch.full((n_rows, n_cols), -1, dtype=torch.int32, device=device),
+                   torch.zeros(n_pages, dtype=torch.int32, device=device),
+                   torch.zeros(n_rows, dtype=torch.int32, device=device), page_size, pool)
+
+    def _call(self, name, *args, stream=None):
+        err = ctypes.create_string_buffer(ERR_CAP)
+        _check(getattr(_paged_lib(), name)(*args, _stream(stream), err, ERR_CAP), err, name)
+
+    def _requests(self, a, b, names):
+        n = a.numel()
+        if n > self.max_requests or (b is not None and b.numel() != n):
+            raise M27BError(f"PageSet: {names}: at most {self.max_requests} requests, as many of each")
+        return _int32(a, names), _int32(b, names), n
+
+    def resize(self, rows, new_lens, stream=None):
+        """Set the rows' lengths (m27b_pages_resize)."""
+        a, b, n = self._requests(rows, new_lens, "rows and new_lens")
+        self._call("m27b_pages_resize", self._ref, self._pools, len(self._pools), a, b, n, self._scratch.data_ptr(),
+                   self.status.data_ptr(), stream=stream)
+
+    def fork(self, src, dst, stream=None):
+        """Make the empty rows dst copies of the rows src (m27b_pages_fork)."""
+        a, b, n = self._requests(src, dst, "src and dst")
+        self._call("m27b_pages_fork", self._ref, self._pools, len(self._pools), a, b, n, self._scratch.data_ptr(),
+                   self.status.data_ptr(), stream=stream)
+
+    def free(self, rows, stream=None):
+        """Empty the rows (m27b_pages_free)."""
+        self._call("m27b_pages_free", self._ref, _int32(rows, "rows"), rows.numel(), stream=stream)
+
+    def compact(self, n_live=None, stream=None):
+        """Move the pages in use to the lowest ids (m27b_pages_compact); n_live, an int32 device tensor, receives their number."""
+        self._call("m27b_pages_compact", self._ref, self._pools, len(self._pools), _int32(n_live, "n_live", 1),
+                   self._scratch.data_ptr(), stream=stream)
+
+    def copy(self, src, dst, stream=None):
+        """Copy page src[i] to page dst[i] in every plane (m27b_pages_copy)."""
+        if src.numel() != dst.numel():
+            raise M27BError("PageSet: src and dst need as many pages")
+        self._call("m27b_pages_copy", self._pools, len(self._pools), self.c.n_pages, _int32(src, "src"), _int32(dst, "dst"),
+                   src.numel(), stream=stream)
+
+    def check(self):
+        """Raise if a request was refused since the last check (reads the device)."""
+        s = int(self.status.item())
+        if s:
+            self.status.zero_()
+            raise M27BError("PageSet: " + {PAGES_FULL: "too few free pages"}.get(s, "bad request (row, length, or a row named twice)"))
