@@ -205,8 +205,8 @@ bool paged_check_kv(const M27BPagedKV *kv, const char *what, char *err, size_t c
     if (kv->n_kv < 1 || kv->n_kv > 1024) return paged_fail(err, cap, "%s: bad n_kv (%d)", what, kv->n_kv);
     if (kv->n_pages < 1 || kv->n_rows < 1 || kv->n_cols < 1)
         return paged_fail(err, cap, "%s: empty cache (%d pages, %d rows of %d)", what, kv->n_pages, kv->n_rows, kv->n_cols);
-    if ((long long)kv->n_cols * kv->page_size > 0x7fffffffll)
-        return paged_fail(err, cap, "%s: n_cols x page_size passes 31 bits", what);
+    if ((long long)kv->n_cols * kv->page_size > 0x3fffffffll)
+        return paged_fail(err, cap, "%s: n_cols x page_size takes 31 bits or more", what);
     if (kv->page_stride < (long long)kv->page_size * kv->n_kv * kv->head_dim || kv->page_stride % 8)
         return paged_fail(err, cap, "%s: page_stride (%lld) must be a multiple of 8, at least a page", what, kv->page_stride);
     if (kv->page_stride > (1ll << 62) / 2 / kv->n_pages)
