@@ -19,16 +19,19 @@
 // them to arrive adds the records in CTA order, so that the result does not
 // depend on who was last.  Every CTA finds its run itself from cu_q and lens.
 //
-// A CTA's roles (6 warps):
-//   * warp 4 streams the key tiles: TMA boxes of 64 values x the positions of
+// A CTA's roles (10 warps):
+//   * warp 8 streams the key tiles: TMA boxes of 64 values x the positions of
 //     a page (or of the tile, if a page is longer), 128-byte swizzle, each lane
 //     one box; a page outside the item's positions is a box past the end of the
 //     pool, which reads zeros;
-//   * warp 5 issues the MMAs: S = Q K^T with Q in TMEM and K (K-major) in shared
+//   * warp 9 issues the MMAs: S = Q K^T with Q in TMEM and K (K-major) in shared
 //     memory, O += P V with P in TMEM and V (N-major) in shared memory;
-//   * warps 0-3 have one row per thread: Q into TMEM, the softmax of S, P back
-//     into TMEM, and at the item's end O / l to global memory.
-// TMEM (512 columns): O | Q | S | P, P.  S is free again once the four warps
+//   * warps 0-7 have half a row per thread, warps w and w + 4 the halves of the
+//     same rows: Q into TMEM, the softmax of S (the two halves tell each other
+//     their maximum), P back into TMEM, and at the item's end O / l to global
+//     memory.  A warp none of whose rows is live (decode: G rows of 128) only
+//     passes the barriers.
+// TMEM (512 columns): O | Q | S | P, P.  S is free again once the warps
 // have loaded it, so the next product runs while they compute; P has two
 // buffers.  Steady state of the tensor pipe: P V of tile t, Q K of tile t + 2,
 // P V of tile t + 1, ...
@@ -62,8 +65,10 @@ struct AttnArgs {
 };
 
 constexpr int PA_ROWS = 128;
-constexpr int PA_THREADS = 192;
-constexpr int PA_PRODUCER = 4, PA_ISSUER = 5;
+constexpr int PA_SOFTMAX = 8;  // softmax warps: two for each 32 rows, each with half of a tile's positions
+constexpr int PA_PRODUCER = PA_SOFTMAX, PA_ISSUER = PA_SOFTMAX + 1;
+constexpr int PA_THREADS = (PA_SOFTMAX + 2) * 32;
+constexpr int PA_JOIN = 1024;  // (row, part) pairs whose factors are held at once when records are joined
 constexpr int PA_MAX_CTAS = 1024;  // counters in the scratch's first 4096 bytes
 constexpr float PA_SLACK = 8.0f;   // growth of the maximum (log2) before m follows
 
@@ -77,7 +82,7 @@ template <int HD> struct PaPlan {
     static_assert(SMEM > MMA_SMEM_MIN && SMEM <= MMA_SMEM_LIMIT, "one CTA per SM");
 };
 
-// floats of a partial record: O[d / 4][row][4], then m and l of the rows
+// floats of a partial record: O[d / 4][row][4], then (m, l) of the rows
 __host__ __device__ constexpr size_t pa_record(int hd) { return (size_t)PA_ROWS * (hd + 2); }
 
 // ---- tensor core helpers ----
@@ -122,6 +127,14 @@ M27B_DI void tmem_st32(uint32_t taddr, const uint32_t *v) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
         "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+M27B_DI void tmem_st16(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
 M27B_DI void tma_load_4d(uint32_t dst, const CUtensorMap *tm, int x, int y, int z, int w, uint64_t *bar) {
@@ -205,7 +218,14 @@ struct PaRun {
     int ctas;             // CTAs that have a run
     int b, j, r, off;     // first item, and units of it that belong to the CTAs before
     long long seq_off, head_units;  // the run's begin within sequence b; units of a kv head of it
+    PaSeq seq;                      // sequence b
 };
+
+// x / y for counts that nearly always fit 32 bits (a 64-bit division is a
+// routine of some hundred cycles, and the prologue has several in a row).
+M27B_DI long long div_count(long long x, long long y) {
+    return (x | y) >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
+}
 
 // The item at hand and its neighbours, walked alike by every role.
 template <int KT>
@@ -220,7 +240,8 @@ struct PaWalk {
 
     M27B_DI PaWalk(const AttnArgs &a_, const PaRun &run, int tq_) : a(a_), tq(tq_) {
         u = run.begin, end = run.end, b = run.b, j = run.j, r = run.r, off = run.off;
-        if (more()) seq(), span();
+        s = run.seq;
+        if (more()) span();
     }
     M27B_DI bool more() const { return u < end; }
     M27B_DI void seq() { s = pa_seq(a, b, tq, false); }
@@ -275,17 +296,20 @@ M27B_DI long long pa_scan(long long v, long long *red, long long *total) {
 template <int KT>
 M27B_DI void pa_find_run(const AttnArgs &a, int tq, PaRun *run, long long *red) {
     const int n = a.bt.n_seq;
-    long long total = 0, u = 0, before = 0, sum;
+    long long total = 0, head = 0, u = 0, before = 0, sum;
+    PaSeq s;
     for (int b0 = 0; b0 < n; b0 += PA_THREADS) {
         const int b = b0 + threadIdx.x;
-        PaSeq s = {0, 0, 0, 0, 0};
+        s = {0, 0, 0, 0, 0};
         if (b < n) s = pa_seq(a, b, tq, blockIdx.x == 0);
-        u = pa_head_units<KT>(s, tq, a.window) * a.kv.n_kv;
+        head = pa_head_units<KT>(s, tq, a.window);
+        u = head * a.kv.n_kv;
         before = pa_scan(u, red, &sum);
         total += sum;
     }
     const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
-    const long long begin = c < ctas ? c * total / ctas : 0, end = c < ctas ? (c + 1) * total / ctas : 0;
+    const long long begin = c < ctas ? div_count(c * total, ctas) : 0,
+                    end = c < ctas ? div_count((c + 1) * total, ctas) : 0;
     if (threadIdx.x == 0) {
         run->total = total, run->ctas = (int)ctas, run->begin = begin, run->end = end;
         run->b = n;
@@ -296,23 +320,25 @@ M27B_DI void pa_find_run(const AttnArgs &a, int tq, PaRun *run, long long *red) 
     for (int b0 = 0; b0 < n && at <= begin; b0 += PA_THREADS) {
         const int b = b0 + threadIdx.x;
         if (n > PA_THREADS) {
-            PaSeq s = {0, 0, 0, 0, 0};
+            s = {0, 0, 0, 0, 0};
             if (b < n) s = pa_seq(a, b, tq, false);
-            u = pa_head_units<KT>(s, tq, a.window) * a.kv.n_kv;
+            head = pa_head_units<KT>(s, tq, a.window);
+            u = head * a.kv.n_kv;
             before = pa_scan(u, red, &sum);
         }
         if (begin >= at + before && begin < at + before + u) {
             run->b = b;
             run->seq_off = begin - at - before;
-            run->head_units = u / a.kv.n_kv;
+            run->head_units = head;
+            run->seq = s;
         }
         at += sum;
         __syncthreads();
     }
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
-        const PaSeq s = pa_seq(a, run->b, tq, false);
-        const long long j = run->seq_off / run->head_units;
+        s = run->seq;
+        const long long j = div_count(run->seq_off, run->head_units);
         long long off = run->seq_off - j * run->head_units;
         int r0 = 0;
         for (;; r0 += 32) {
@@ -339,10 +365,84 @@ M27B_DI void pa_find_run(const AttnArgs &a, int tq, PaRun *run, long long *red) 
 struct PaShared {
     PaRun run;
     long long red[PA_THREADS / 32];
+    float half[2][2][PA_ROWS];  // what the two warps of a row tell each other, by turns
+    float2 join[PA_JOIN];
     uint32_t tmem;
     int abort;
     int last;
 };
+
+// Add up the np records of an item of CTAs c0, c0 + 1, ... and write its rows;
+// the softmax warps of the CTA that arrived last.  Rows are taken so many at a
+// time that their parts' m and l fit `join`, fetched in one round trip; a
+// part's factor is 2^(m - max) / sum.  Then four quadruples of values x four
+// parts a thread are in flight.
+template <int HD, bool BF, class Walk, class Sync>
+M27B_DI bool pa_join(const AttnArgs &a, const Walk &w, int c0, int np, int rows, int G, int tq, float2 *join, int tid,
+                     Sync all_here) {
+    constexpr int NT = 32 * PA_SOFTMAX;
+    auto record = [&](int x) { return a.part + (size_t)(2 * (c0 + x) + (x == 0 ? 1 : 0)) * pa_record(HD); };
+    const int at_once = min(rows, PA_JOIN / np);
+    for (int r0 = 0; r0 < rows; r0 += at_once) {
+        const int nr = min(at_once, rows - r0);
+        for (int e = tid; e < nr * np; e += NT) {
+            const int x = e / nr;
+            join[e] = __ldcg((const float2 *)(record(x) + (size_t)PA_ROWS * HD) + r0 + e - x * nr);
+        }
+        if (!all_here()) return false;
+        for (int r = tid; r < nr; r += NT) {
+            float mx = -INFINITY, ls = 0.0f;
+            for (int x = 0; x < np; ++x) mx = fmaxf(mx, join[x * nr + r].x);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            for (int x = 0; x < np; ++x) {
+                const float2 ml = join[x * nr + r];
+                const float f = ex2(ml.x - ref);
+                join[x * nr + r].x = f;
+                ls = fmaf(f, ml.y, ls);
+            }
+            const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
+            for (int x = 0; x < np; ++x) join[x * nr + r].x *= inv;
+            if (a.lse)
+                a.lse[(w.s.q_lo + w.r * tq + (r0 + r) / G) * (long long)a.n_q + w.j * G + (r0 + r) % G] =
+                    ls > 0.0f ? 0.69314718055994530942f * (mx + log2f(ls)) : -INFINITY;
+        }
+        if (!all_here()) return false;
+        for (int e0 = tid; e0 < nr * (HD / 4); e0 += 4 * NT) {
+            float4 o[4] = {};
+            int rr[4], dd[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) dd[g] = (e0 + NT * g) / nr, rr[g] = e0 + NT * g - dd[g] * nr;
+            for (int x0 = 0; x0 < np; x0 += 4) {
+                float4 y[4][4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float4 *rx = (const float4 *)record(x0 + x) + r0;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        y[g][x] = x0 + x < np && dd[g] < HD / 4 ? __ldcg(rx + (size_t)dd[g] * PA_ROWS + rr[g])
+                                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float f = x0 + x < np ? join[(x0 + x) * nr + rr[g]].x : 0.0f;
+                        o[g].x = fmaf(f, y[g][x].x, o[g].x), o[g].y = fmaf(f, y[g][x].y, o[g].y);
+                        o[g].z = fmaf(f, y[g][x].z, o[g].z), o[g].w = fmaf(f, y[g][x].w, o[g].w);
+                    }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (dd[g] >= HD / 4) continue;
+                const long long tk = w.s.q_lo + w.r * tq + (r0 + rr[g]) / G;
+                *(uint2 *)((uint16_t *)a.out + tk * a.out_stride + (long long)(w.j * G + (r0 + rr[g]) % G) * HD + 4 * dd[g]) =
+                    make_uint2(Half16<BF>::down(o[g].x, o[g].y), Half16<BF>::down(o[g].z, o[g].w));
+            }
+        }
+        if (r0 + at_once < rows && !all_here()) return false;  // the factors are about to be replaced
+    }
+    return true;
+}
 
 template <int HD, bool BF>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -353,7 +453,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     uint8_t *smem = (uint8_t *)(((uintptr_t)pa_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = (uint64_t *)(smem + (size_t)ST * 2 * TILE);
     uint64_t *kfull = bars, *vfull = kfull + ST, *empty = vfull + ST, *qfull = empty + ST, *sfull = qfull + 1,
-             *sfree = sfull + 1, *pfull = sfree + 1, *pdone = pfull + 2, *drain = pdone + 2, *meet = drain + 1;
+             *sfree = sfull + 1, *pfull = sfree + 1, *pdone = pfull + 2, *drain = pdone + 2, *meet = drain + 1, *pair = meet + 1;
     __shared__ PaShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.n_q / a.kv.n_kv, tq = PA_ROWS / G;
@@ -365,15 +465,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             mbar_init(&vfull[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(qfull, 4);
+        mbar_init(qfull, PA_SOFTMAX);
         mbar_init(sfull, 1);
-        mbar_init(sfree, 4);
+        mbar_init(sfree, PA_SOFTMAX);
+        for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&pfull[i], 4);
+            mbar_init(&pfull[i], PA_SOFTMAX);
             mbar_init(&pdone[i], 1);
         }
         mbar_init(drain, 1);
-        mbar_init(meet, 4);
+        mbar_init(meet, PA_SOFTMAX);
         sh.abort = 0;
         fence_mbar_init();
     }
@@ -484,35 +585,51 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             mbar_wait_bounded(drain, 0u, a.status, 5);
         }
         __syncwarp();
-    } else if (warp < 4) {
-        const uint32_t lane_base = tmem + ((uint32_t)(32 * warp) << 16);
+    } else {
+        // row = TMEM lane; this thread has positions [half KH, half KH + KH) of
+        // each tile, and columns [half HD / 2, ..) of O
+        constexpr int KH = KT / 2;
+        const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
         const float c = a.scale * 1.44269504088896340736f;  // log2 e
-        int t = 0, met = 0;
+        int t = 0, met = 0, told = 0;
         bool ok = true;
-        // the four warps wait for one another (bounded: a warp that gave up never comes)
+        // the softmax warps wait for one another (bounded: a warp that gave up never comes)
         auto all_here = [&] {
             __syncwarp();
             if (lane == 0) mbar_arrive(meet);
             return warp_wait_or_abort(meet, (uint32_t)(met++ & 1), abort, a.status);
         };
+        // this row's value of the other half
+        auto other = [&](float mine, float &theirs) {
+            const int turn = told++ & 1;
+            sh.half[turn][half][row] = mine;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pair[quarter]);
+            const bool here = warp_wait_or_abort(&pair[quarter], (uint32_t)turn, abort, a.status);
+            theirs = *(volatile float *)&sh.half[turn][half ^ 1][row];
+            return here;
+        };
         for (; ok && w.more(); w.next()) {
-            const int n = w.tiles(), i = w.r * tq + tid / G, h = w.j * G + tid % G;
-            const bool live = tid < tq * G && i < w.s.q_n;
-            const int hi = live ? w.s.base + i + 1 : 0;
-            const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
+            const int n = w.tiles(), i = w.r * tq + row / G, h = w.j * G + row % G;
+            const int rows = min(tq, w.s.q_n - w.r * tq) * G;
+            const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
+            // a dead row's scores are garbage that no one reads
+            const int hi = live ? w.s.base + i + 1 : 0x7fffffff;
+            const int lo = live && a.window > 0 ? max(0, hi - a.window) : 0;
             float m = -INFINITY, l = 0.0f;  // m in units of c s
             if (n > 0) {
-                // Q of this row into TMEM (its last product has been read as S)
-                const uint16_t *qp = (const uint16_t *)a.q + (long long)(w.s.q_lo + i) * a.q_stride + (long long)h * HD;
+                // half of this row's Q into TMEM (its last product has been read as S)
+                const uint16_t *qp = (const uint16_t *)a.q + (long long)(w.s.q_lo + i) * a.q_stride + (long long)h * HD + half * (HD / 2);
 #pragma unroll
                 for (int x = 0; x < HD / 64; ++x) {
-                    uint32_t v[32];
+                    uint32_t v[16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint4 y = live ? __ldg((const uint4 *)(qp + 64 * x) + e) : make_uint4(0, 0, 0, 0);
+                    for (int e = 0; e < 4; ++e) {
+                        const uint4 y = live ? __ldg((const uint4 *)(qp + 32 * x) + e) : make_uint4(0, 0, 0, 0);
                         v[4 * e] = y.x, v[4 * e + 1] = y.y, v[4 * e + 2] = y.z, v[4 * e + 3] = y.w;
                     }
-                    tmem_st32(lane_base + L::Q + 32 * x, v);
+                    tmem_st16(lane_base + L::Q + half * (HD / 4) + 16 * x, v);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -521,77 +638,73 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             for (int k = 0; k < n; ++k, ++t) {
                 const int x0 = (w.first() + k) * KT;
-                if (!warp_wait_or_abort(sfull, (uint32_t)(t & 1), abort, a.status)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                float s[KT];
+                if (!(ok = warp_wait_or_abort(sfull, (uint32_t)(t & 1), abort, a.status))) break;
+                if (idle) {
+                    if (lane == 0) mbar_arrive(sfree);
+                } else {
+                    tc_fence_after();
+                    float s[KH];
 #pragma unroll
-                for (int x = 0; x < KT / 32; ++x) tmem_ld32(lane_base + L::S + 32 * x, (uint32_t *)s + 32 * x);
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sfree);
-                if (__any_sync(0xffffffffu, x0 < lo || x0 + KT > hi)) {
+                    for (int x = 0; x < KH / 32; ++x) tmem_ld32(lane_base + L::S + half * KH + 32 * x, (uint32_t *)s + 32 * x);
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sfree);
+                    const int xh = x0 + half * KH;
+                    if (__any_sync(0xffffffffu, xh < lo || xh + KH > hi)) {
 #pragma unroll
-                    for (int x = 0; x < KT; ++x)
-                        if (x0 + x < lo || x0 + x >= hi) s[x] = -INFINITY;
-                }
-                float top = s[0];
-#pragma unroll
-                for (int x = 1; x < KT; ++x) top = fmaxf(top, s[x]);
-                top *= c;
-                if (__any_sync(0xffffffffu, top > m + PA_SLACK)) {
-                    const float to = top > m + PA_SLACK ? top : m;
-                    const float f = m == -INFINITY ? 1.0f : ex2(m - to);
-                    m = to;
-                    l *= f;
-                    if (k > 0) {
-                        // O of the tiles so far, once their products are done
-                        if (!warp_wait_or_abort(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        for (int x = 0; x < HD / 32; ++x) {
-                            uint32_t v[32];
-                            tmem_ld32(lane_base + L::O + 32 * x, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            tmem_st32(lane_base + L::O + 32 * x, v);
-                        }
-                        tmem_wait_st();
+                        for (int x = 0; x < KH; ++x)
+                            if (xh + x < lo || xh + x >= hi) s[x] = -INFINITY;
                     }
-                }
-                const float mm = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                // P's buffer is free once the product of two tiles ago is done
-                if (t >= 2 && !warp_wait_or_abort(&pdone[t & 1], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status)) {
-                    ok = false;
-                    break;
-                }
+                    float tops[4] = {s[0], s[1], s[2], s[3]}, theirs;
 #pragma unroll
-                for (int x = 0; x < KT / 64; ++x) {
-                    uint32_t v[32];
+                    for (int x = 4; x < KH; ++x) tops[x & 3] = fmaxf(tops[x & 3], s[x]);
+                    const float mine = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    if (!(ok = other(mine, theirs))) break;
+                    const float top = c * fmaxf(mine, theirs);
+                    if (__any_sync(0xffffffffu, top > m + PA_SLACK)) {
+                        const float to = top > m + PA_SLACK ? top : m;
+                        const float f = m == -INFINITY ? 1.0f : ex2(m - to);
+                        m = to;
+                        l *= f;
+                        if (k > 0) {
+                            // this half's columns of O, once the products so far are done
+                            if (!(ok = warp_wait_or_abort(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status)))
+                                break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int x = 0; x < HD / 64; ++x) {
+                                uint32_t v[32];
+                                tmem_ld32(lane_base + L::O + half * (HD / 2) + 32 * x, v);
+                                tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float p0 = ex2(fmaf(s[64 * x + 2 * e], c, -mm)), p1 = ex2(fmaf(s[64 * x + 2 * e + 1], c, -mm));
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                                tmem_st32(lane_base + L::O + half * (HD / 2) + 32 * x, v);
+                            }
+                            tmem_wait_st();
+                        }
+                    }
+                    const float mm = m == -INFINITY ? 0.0f : m;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    uint32_t p[KH / 2];
+#pragma unroll
+                    for (int e = 0; e < KH / 2; ++e) {
+                        const float p0 = ex2(fmaf(s[2 * e], c, -mm)), p1 = ex2(fmaf(s[2 * e + 1], c, -mm));
                         sum[e & 3] += p0 + p1;
-                        v[e] = Half16<BF>::down(p0, p1);
+                        p[e] = Half16<BF>::down(p0, p1);
                     }
-                    tmem_st32(lane_base + L::P + (t & 1) * (KT / 2) + 32 * x, v);
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    // P's buffer is free once the product of two tiles ago is done
+                    if (t >= 2 && !(ok = warp_wait_or_abort(&pdone[t & 1], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status))) break;
+                    const uint32_t pc = lane_base + L::P + (t & 1) * (KT / 2) + half * (KH / 2);
+                    if constexpr (KH == 64) tmem_st32(pc, p);
+                    else tmem_st16(pc, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 // values of positions that no row of the item sees
                 if (x0 < w.sp.lo || x0 + KT > w.sp.hi) {
-                    if (!warp_wait_or_abort(&vfull[t % ST], (uint32_t)((t / ST) & 1), abort, a.status)) {
-                        ok = false;
-                        break;
-                    }
+                    if (!(ok = warp_wait_or_abort(&vfull[t % ST], (uint32_t)((t / ST) & 1), abort, a.status))) break;
                     uint8_t *v = smem + (size_t)(t % ST) * 2 * TILE + TILE;
-                    for (int e = tid; e < KT * NCH * 8; e += 128) {
+                    for (int e = tid; e < KT * NCH * 8; e += 32 * PA_SOFTMAX) {
                         const int x = (e >> 3) % KT;
                         if (x0 + x < w.sp.lo || x0 + x >= w.sp.hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
                     }
@@ -604,20 +717,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             if (!ok) break;
             if (n > 0) {
-                if (!warp_wait_or_abort(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status)) {
-                    ok = false;
-                    break;
-                }
+                if (!(ok = warp_wait_or_abort(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status))) break;
                 tc_fence_after();
+            }
+            if (!idle) {
+                float theirs;
+                if (!(ok = other(l, theirs))) break;
+                l = half ? theirs + l : l + theirs;
             }
             const long long tok = w.s.q_lo + i;
             if (w.whole()) {
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                uint16_t *op = (uint16_t *)a.out + tok * a.out_stride + (long long)h * HD;
-                for (int x = 0; x < HD / 32; ++x) {
+                uint16_t *op = (uint16_t *)a.out + tok * a.out_stride + (long long)h * HD + half * (HD / 2);
+#pragma unroll 1
+                for (int x = 0; x < (idle ? 0 : HD / 64); ++x) {
                     uint32_t v[32];
                     if (n > 0) {
-                        tmem_ld32(lane_base + L::O + 32 * x, v);
+                        tmem_ld32(lane_base + L::O + half * (HD / 2) + 32 * x, v);
                         tmem_wait_ld();
                     }
                     if (live)
@@ -632,30 +748,28 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                             *((uint4 *)(op + 32 * x) + e) = make_uint4(y[0], y[1], y[2], y[3]);
                         }
                 }
-                if (live && a.lse)
+                if (live && a.lse && half == 0)
                     a.lse[tok * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
                 tc_fence_before();
             } else {
                 // this CTA's part of the item; the last of the item's CTAs adds them up
                 const long long U = w.u - w.off;
-                const int c0 = (int)(((U + 1) * sh.run.ctas + sh.run.total - 1) / sh.run.total) - 1;
-                const int c1 = (int)(((U + w.sp.units()) * sh.run.ctas + sh.run.total - 1) / sh.run.total) - 1;
+                const int c0 = (int)div_count((U + 1) * sh.run.ctas + sh.run.total - 1, sh.run.total) - 1;
+                const int c1 = (int)div_count((U + w.sp.units()) * sh.run.ctas + sh.run.total - 1, sh.run.total) - 1;
                 const int me = blockIdx.x;
                 float *rec = a.part + (size_t)(2 * me + (me == c0 ? 1 : 0)) * pa_record(HD);
-                for (int x = 0; x < HD / 32; ++x) {
+#pragma unroll 1
+                for (int x = 0; x < (idle ? 0 : HD / 64); ++x) {
                     uint32_t v[32];
-                    tmem_ld32(lane_base + L::O + 32 * x, v);
+                    tmem_ld32(lane_base + L::O + half * (HD / 2) + 32 * x, v);
                     tmem_wait_ld();
                     if (live)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            __stcg((uint4 *)rec + (size_t)(8 * x + e) * PA_ROWS + tid,
+                            __stcg((uint4 *)rec + (size_t)(half * (HD / 8) + 8 * x + e) * PA_ROWS + row,
                                    make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
                 }
-                if (live) {
-                    __stcg(rec + (size_t)PA_ROWS * HD + tid, m);
-                    __stcg(rec + (size_t)PA_ROWS * (HD + 1) + tid, l);
-                }
+                if (live && half == 0) __stcg((float2 *)(rec + (size_t)PA_ROWS * HD) + row, make_float2(m, l));
                 tc_fence_before();
                 __threadfence();
                 if (!(ok = all_here())) break;
@@ -666,35 +780,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     sh.last = last;
                 }
                 if (!(ok = all_here())) break;
-                if (*(volatile int *)&sh.last) {
-                    const int rows = min(tq, w.s.q_n - w.r * tq) * G;
-                    auto record = [&](int cta) { return a.part + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * pa_record(HD); };
-                    for (int e = tid; e < rows * (HD / 4); e += 128) {
-                        const int row = e % rows, d4 = e / rows;
-                        float mx = -INFINITY;
-                        for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, __ldcg(record(x) + (size_t)PA_ROWS * HD + row));
-                        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        float ls = 0.0f;
-                        for (int x = c0; x <= c1; ++x) {
-                            const float *rx = record(x);
-                            const float mr = __ldcg(rx + (size_t)PA_ROWS * HD + row);
-                            const float f = mr == -INFINITY ? 0.0f : ex2(mr - mx);
-                            ls = fmaf(f, __ldcg(rx + (size_t)PA_ROWS * (HD + 1) + row), ls);
-                            const float4 y = __ldcg((const float4 *)rx + (size_t)d4 * PA_ROWS + row);
-                            if (f > 0.0f) {
-                                o.x = fmaf(f, y.x, o.x), o.y = fmaf(f, y.y, o.y);
-                                o.z = fmaf(f, y.z, o.z), o.w = fmaf(f, y.w, o.w);
-                            }
-                        }
-                        const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
-                        const long long tk = w.s.q_lo + w.r * tq + row / G;
-                        const int hh = w.j * G + row % G;
-                        *(uint2 *)((uint16_t *)a.out + tk * a.out_stride + (long long)hh * HD + 4 * d4) =
-                            make_uint2(Half16<BF>::down(o.x * inv, o.y * inv), Half16<BF>::down(o.z * inv, o.w * inv));
-                        if (d4 == 0 && a.lse)
-                            a.lse[tk * a.n_q + hh] = ls > 0.0f ? 0.69314718055994530942f * (mx + log2f(ls)) : -INFINITY;
-                    }
-                }
+                if (*(volatile int *)&sh.last) ok = pa_join<HD, BF>(a, w, c0, c1 - c0 + 1, rows, G, tq, sh.join, tid, all_here);
             }
         }
     }

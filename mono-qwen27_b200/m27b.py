@@ -8,6 +8,8 @@ libm27b.so is missing or fails to load, every call raises.
 """
 import ctypes
 import os
+import struct
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libm27b.so")
@@ -766,7 +768,7 @@ M27B_VERIFY_MAX = 16
 # --------------------------------------------------------------------------
 # paged key/value cache (include/m27b_paged.h)
 
-BF16 = 30
+BF16, I32 = 30, 26
 ROPE_NONE, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
 PAGES_FULL, PAGES_BAD = 1, 2
 
@@ -779,29 +781,18 @@ class _PagedKV(ctypes.Structure):
                 ("page_stride", ctypes.c_longlong)]
 
 
-class _PagedBatch(ctypes.Structure):
-    """M27BPagedBatch"""
-    _fields_ = [("cu_q", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("rows", ctypes.c_void_p),
-                ("n_seq", ctypes.c_int), ("n_tok", ctypes.c_int)]
+# Small by-reference arguments of the calls a decode step makes, packed as C
+# lays them out (a bytes object is passed as the pointer to it; packing one
+# takes a third of the time of filling a ctypes.Structure).
+_PagedBatch = struct.Struct("@PPPii")               # M27BPagedBatch: cu_q, lens, rows, n_seq, n_tok
+_Rope = struct.Struct("@PiiiP")                     # M27BRope: table, n_pos, n_rot, interleaved, positions
+_Heads = struct.Struct("@PPPqqqIiPPf4x")            # M27BHeads: q, k, v, strides, src_type, n_q, q_norm, k_norm, eps
 
 
 class _RopeScaling(ctypes.Structure):
     """M27BRopeScaling"""
     _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_float), ("original_ctx", ctypes.c_int),
                 ("beta_fast", ctypes.c_float), ("beta_slow", ctypes.c_float), ("attn_factor", ctypes.c_float)]
-
-
-class _Rope(ctypes.Structure):
-    """M27BRope"""
-    _fields_ = [("table", ctypes.c_void_p), ("n_pos", ctypes.c_int), ("n_rot", ctypes.c_int),
-                ("interleaved", ctypes.c_int), ("positions", ctypes.c_void_p)]
-
-
-class _Heads(ctypes.Structure):
-    """M27BHeads"""
-    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_longlong),
-                ("k_stride", ctypes.c_longlong), ("v_stride", ctypes.c_longlong), ("src_type", ctypes.c_uint32),
-                ("n_q", ctypes.c_int), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
 
 
 class _Pages(ctypes.Structure):
@@ -817,18 +808,22 @@ class _PagePool(ctypes.Structure):
                 ("page_stride", ctypes.c_size_t), ("page_bytes", ctypes.c_size_t)]
 
 
+_paged = None
+
+
 def _paged_lib():
+    global _paged
+    if _paged is not None and _paged is _lib:
+        return _paged
     L = lib()
-    if getattr(L, "_paged_sigs", False):
-        return L
     vp, cp, sz, i32, ll, b = (ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_longlong,
                               ctypes.c_bool)
-    kv, bt, pg, pool = (ctypes.POINTER(t) for t in (_PagedKV, _PagedBatch, _Pages, _PagePool))
+    kv, pg, pool = (ctypes.POINTER(t) for t in (_PagedKV, _Pages, _PagePool))
     sig = {
         "m27b_rope_table": (b, [vp, i32, i32, ctypes.c_double, ctypes.POINTER(_RopeScaling), vp, cp, sz]),
-        "m27b_rope_append": (b, [kv, bt, ctypes.POINTER(_Rope), ctypes.POINTER(_Heads), vp, ll, vp, cp, sz]),
+        "m27b_rope_append": (b, [kv, cp, cp, cp, vp, ll, vp, cp, sz]),
         "m27b_paged_attn_scratch_bytes": (sz, [i32, i32, i32]),
-        "m27b_paged_attn": (b, [kv, bt, vp, ll, i32, ctypes.c_float, i32, vp, ll, vp, vp, vp, cp, sz]),
+        "m27b_paged_attn": (b, [kv, cp, vp, ll, i32, ctypes.c_float, i32, vp, ll, vp, vp, vp, cp, sz]),
         "m27b_pages_scratch_bytes": (sz, [i32, i32, i32]),
         "m27b_pages_resize": (b, [pg, pool, i32, vp, vp, i32, vp, vp, vp, cp, sz]),
         "m27b_pages_fork": (b, [pg, pool, i32, vp, vp, i32, vp, vp, vp, cp, sz]),
@@ -840,36 +835,65 @@ def _paged_lib():
         f = getattr(L, name)
         f.restype = res
         f.argtypes = args
-    L._paged_sigs = True
+    _paged = L
     return L
 
 
+_types = {}  # torch type -> ggml code, filled at the first use (torch is imported late)
+
+
 def _paged_type(dtype):
-    import torch
-    t = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}.get(dtype)
+    if not _types:
+        import torch
+        _types.update({torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.int32: I32})
+    t = _types.get(dtype)
     if t is None:
-        raise M27BError(f"paged cache: unsupported type {dtype}")
+        raise M27BError(f"paged cache: unsupported type {dtype} (f16, bf16; f32 and int32 where named)")
     return t
 
 
-def _int32(t, what, n=None):
-    """The data pointer of a contiguous device int32 tensor (None passes)."""
+def _f32(t):
+    """A contiguous fp32 device tensor?"""
+    return t.is_cuda and _paged_type(t.dtype) == F32 and t.is_contiguous()
+
+
+# A decode step makes these calls once per layer on a few rows, so what they
+# cost on the host counts: plain attribute reads, one error buffer per thread,
+# the current stream's handle without a Stream object.
+_tls = threading.local()
+
+
+def _err():
+    try:
+        return _tls.err
+    except AttributeError:
+        _tls.err = ctypes.create_string_buffer(ERR_CAP)
+        return _tls.err
+
+
+def _raw_stream(stream):
+    if stream is not None:
+        return stream.cuda_stream
     import torch
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _int32(t, what, n=0):
+    """The data pointer of a contiguous device int32 tensor (0 for None)."""
     if t is None:
-        return None
-    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() < n):
+        return 0
+    if not t.is_cuda or _paged_type(t.dtype) != I32 or t.numel() < n or not t.is_contiguous():
         raise M27BError(f"{what} must be a contiguous int32 device tensor" + (f" of at least {n} values" if n else ""))
     return t.data_ptr()
 
 
 def _token_heads(t, what, n_tok, n_head, head_dim, dtype):
     """(pointer, token stride) of [n_tok, n_head, head_dim] rows whose heads are contiguous."""
-    if t.dim() != 3 or t.shape[0] != n_tok or t.shape[1] != n_head or t.shape[2] != head_dim or t.dtype != dtype \
-            or not t.is_cuda:
+    if t.shape != (n_tok, n_head, head_dim) or t.dtype != dtype or not t.is_cuda:
         raise M27BError(f"{what} must be a device tensor [{n_tok}, {n_head}, {head_dim}] of {dtype} "
                         f"(got {list(t.shape)} of {t.dtype})")
     s = t.stride()
-    if (s[2] != 1 and head_dim > 1) or (s[1] != head_dim and n_head > 1):
+    if s[2] != 1 or (s[1] != head_dim and n_head > 1):
         raise M27BError(f"{what}: a token's heads must be contiguous (strides {s})")
     return t.data_ptr(), s[0] if n_tok > 1 else n_head * head_dim
 
@@ -904,8 +928,8 @@ def _batch(kv, cu_q, lens, rows, n_tok):
     n_seq = cu_q.numel() - 1
     if n_seq < 0:
         raise M27BError("cu_q needs n_seq + 1 values")
-    return _PagedBatch(_int32(cu_q, "cu_q"), _int32(lens, "lens", kv.c.n_rows if rows is not None else n_seq),
-                       _int32(rows, "rows", n_seq), n_seq, n_tok)
+    return _PagedBatch.pack(_int32(cu_q, "cu_q"), _int32(lens, "lens", kv.c.n_rows if rows is not None else n_seq),
+                            _int32(rows, "rows", n_seq), n_seq, n_tok)
 
 
 def rope_table(n_pos, n_rot, theta, kind=ROPE_NONE, factor=1.0, original_ctx=0, beta_fast=32.0, beta_slow=1.0,
@@ -929,27 +953,29 @@ def rope_append(kv, q, k, v, cu_q, lens, rope, q_out, interleaved=False, q_norm=
     the cache (m27b_rope_append).  cu_q [n_seq + 1]: each sequence's token
     rows; lens: positions of each table row, the new ones included; rope: a
     table of rope_table.  q may be None (append only)."""
-    import torch
-    n_tok, n_q = k.shape[0], 0 if q is None else q.shape[1]
-    kp, ks = _token_heads(k, "k", n_tok, kv.n_kv, kv.head_dim, k.dtype)
-    vp, vs = _token_heads(v, "v", n_tok, kv.n_kv, kv.head_dim, k.dtype)
-    qp, qs, op, os_ = None, 0, None, 0
+    dt, n_kv, hd = k.dtype, kv.n_kv, kv.head_dim
+    n_tok = k.shape[0]
+    kp, ks = _token_heads(k, "k", n_tok, n_kv, hd, dt)
+    vp, vs = _token_heads(v, "v", n_tok, n_kv, hd, dt)
+    n_q = qp = op = qs = os_ = 0
     if q is not None:
-        qp, qs = _token_heads(q, "q", n_tok, n_q, kv.head_dim, k.dtype)
-        op, os_ = _token_heads(q_out, "q_out", n_tok, n_q, kv.head_dim, kv.dtype)
-    if rope.dim() != 3 or rope.shape[2] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
+        n_q = q.shape[1]
+        qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt)
+        op, os_ = _token_heads(q_out, "q_out", n_tok, n_q, hd, kv.dtype)
+    n_pos, half, two = rope.shape
+    if two != 2 or not _f32(rope):
         raise M27BError("rope must be an fp32 table [n_pos, n_rot / 2, 2]")
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != kv.head_dim or not w.is_contiguous()):
-            raise M27BError(f"{name} must be {kv.head_dim} fp32 values")
+    if (q_norm is not None and (q_norm.numel() != hd or not _f32(q_norm))) or \
+            (k_norm is not None and (k_norm.numel() != hd or not _f32(k_norm))):
+        raise M27BError(f"q_norm and k_norm must be {hd} fp32 values on the device")
     bt = _batch(kv, cu_q, lens, rows, n_tok)
-    rp = _Rope(rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], 1 if interleaved else 0,
-               _int32(positions, "positions", n_tok))
-    hd = _Heads(qp, kp, vp, qs, ks, vs, _paged_type(k.dtype), n_q, q_norm.data_ptr() if q_norm is not None else None,
-                k_norm.data_ptr() if k_norm is not None else None, eps)
-    err = ctypes.create_string_buffer(ERR_CAP)
-    _check(_paged_lib().m27b_rope_append(kv._ref, ctypes.byref(bt), ctypes.byref(rp), ctypes.byref(hd), op, os_,
-                                         _stream(stream), err, ERR_CAP), err, "m27b_rope_append")
+    rp = _Rope.pack(rope.data_ptr(), n_pos, 2 * half, 1 if interleaved else 0, _int32(positions, "positions", n_tok))
+    h = _Heads.pack(qp, kp, vp, qs, ks, vs, _paged_type(dt), n_q, 0 if q_norm is None else q_norm.data_ptr(),
+                    0 if k_norm is None else k_norm.data_ptr(), eps)
+    err = _err()
+    if not _paged_lib().m27b_rope_append(kv._ref, bt, rp, h, op, os_, _raw_stream(stream), err,
+                                         ERR_CAP):
+        _check(False, err, "m27b_rope_append")
     return q_out
 
 
@@ -968,20 +994,23 @@ def paged_attn(kv, q, cu_q, lens, out, scratch, scale=None, window=0, lse=None, 
     lens - 1; window > 0 limits a token to the last `window` positions; lse
     [n_tok, n_q] fp32 receives the log sum of exponentials.  scale defaults to
     1 / sqrt(hd)."""
-    import torch
-    n_tok, n_q = q.shape[0], q.shape[1]
-    qp, qs = _token_heads(q, "q", n_tok, n_q, kv.head_dim, kv.dtype)
-    op, os_ = _token_heads(out, "out", n_tok, n_q, kv.head_dim, kv.dtype)
+    hd, dt = kv.head_dim, kv.dtype
+    n_tok, n_q, _ = q.shape
+    qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt)
+    op, os_ = _token_heads(out, "out", n_tok, n_q, hd, dt)
     L = _paged_lib()
-    if scratch.numel() * scratch.element_size() < L.m27b_paged_attn_scratch_bytes(n_q, kv.n_kv, kv.head_dim):
-        raise M27BError("paged_attn: scratch is too small for these heads")
-    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != n_tok * n_q or not lse.is_contiguous()):
-        raise M27BError(f"lse must be {n_tok} x {n_q} fp32 values")
+    if not scratch.is_cuda or scratch.numel() < L.m27b_paged_attn_scratch_bytes(n_q, kv.n_kv, hd):
+        raise M27BError("paged_attn: scratch is too small for these heads (use paged_attn_scratch)")
+    lp = None
+    if lse is not None:
+        if lse.numel() != n_tok * n_q or not _f32(lse):
+            raise M27BError(f"lse must be {n_tok} x {n_q} fp32 values on the device")
+        lp = lse.data_ptr()
     bt = _batch(kv, cu_q, lens, rows, n_tok)
-    err = ctypes.create_string_buffer(ERR_CAP)
-    _check(L.m27b_paged_attn(kv._ref, ctypes.byref(bt), qp, qs, n_q, kv.head_dim ** -0.5 if scale is None else scale,
-                             window, op, os_, lse.data_ptr() if lse is not None else None, scratch.data_ptr(),
-                             _stream(stream), err, ERR_CAP), err, "m27b_paged_attn")
+    err = _err()
+    if not L.m27b_paged_attn(kv._ref, bt, qp, qs, n_q, hd ** -0.5 if scale is None else scale, window, op, os_, lp,
+                             scratch.data_ptr(), _raw_stream(stream), err, ERR_CAP):
+        _check(False, err, "m27b_paged_attn")
     return out
 
 
@@ -1030,8 +1059,9 @@ class PageSet:
                    torch.zeros(n_rows, dtype=torch.int32, device=device), page_size, pool)
 
     def _call(self, name, *args, stream=None):
-        err = ctypes.create_string_buffer(ERR_CAP)
-        _check(getattr(_paged_lib(), name)(*args, _stream(stream), err, ERR_CAP), err, name)
+        err = _err()
+        if not getattr(_paged_lib(), name)(*args, _raw_stream(stream), err, ERR_CAP):
+            _check(False, err, name)
 
     def _requests(self, a, b, names):
         n = a.numel()

@@ -15,7 +15,7 @@ def _kv(m, **kw):
 def _batch(m, **kw):
     d = dict(cu_q=0x40000, lens=0x50000, rows=None, n_seq=2, n_tok=2)
     d.update(kw)
-    return m._PagedBatch(**d)
+    return m._PagedBatch.pack(*(v or 0 for v in d.values()))
 
 
 BAD_KV = [(dict(k=None), "null pool"), (dict(table=None), "null pool"), (dict(v=0x20008), "16-byte"), (dict(type=0), "f16 or bf16"),
@@ -29,7 +29,7 @@ BAD_BATCH = [(dict(cu_q=None), "null batch"), (dict(lens=None), "null batch"), (
 
 def _attn(m, kv=None, bt=None, q=0x60000, qs=512, n_q=4, scale=1.0, window=0, out=0x70000, os=512, scr=0x80000):
     m._paged_lib()
-    return m.call_raw("m27b_paged_attn", ctypes.byref(kv or _kv(m)), ctypes.byref(bt or _batch(m)), q, qs, n_q, scale,
+    return m.call_raw("m27b_paged_attn", ctypes.byref(kv or _kv(m)), bt or _batch(m), q, qs, n_q, scale,
                       window, out, os, None, scr, None)
 
 
@@ -76,8 +76,8 @@ def _rope(m, kv=None, rope=None, heads=None, out=0x90000, os=512):
     h = dict(q=0x60000, k=0x61000, v=0x62000, q_stride=1024, k_stride=1024, v_stride=1024, src_type=m.F32, n_q=4,
              q_norm=None, k_norm=None, eps=1e-6)
     h.update(heads or {})
-    return m.call_raw("m27b_rope_append", ctypes.byref(kv or _kv(m)), ctypes.byref(_batch(m)), ctypes.byref(m._Rope(**r)),
-                      ctypes.byref(m._Heads(**h)), out, os, None)
+    return m.call_raw("m27b_rope_append", ctypes.byref(kv or _kv(m)), _batch(m), m._Rope.pack(*(v or 0 for v in r.values())),
+                      m._Heads.pack(*(v or 0 for v in h.values())), out, os, None)
 
 
 @pytest.mark.parametrize("kw,needle", [
