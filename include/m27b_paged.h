@@ -126,9 +126,8 @@ M27B_API bool m27b_rope_append(const M27BPagedKV *kv, const M27BPagedBatch *batc
 
 /* ---- attention ---- */
 
-/* Scratch of m27b_paged_attn: its first 4096 bytes (arrival counters) start
- * zeroed and every call leaves them so; calls that may overlap need one each.
- * 0 for an invalid shape. */
+/* Scratch of m27b_paged_attn, contents free; calls that may overlap need one
+ * each.  0 for an invalid shape. */
 M27B_API size_t m27b_paged_attn_scratch_bytes(int n_q, int n_kv, int head_dim);
 
 /* out[t][h] = softmax(scale * q[t][h] . K) V over the positions that token t

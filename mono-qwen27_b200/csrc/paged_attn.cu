@@ -11,30 +11,39 @@
 // Work.  An item is 128 rows (128 / G tokens x the G heads of a kv head, so
 // that a key tile is read once for the group) of one sequence and kv head,
 // over the key tiles its rows see; a unit is one item's work on one key tile.
-// All items' units in a row are cut into one even run per CTA (one CTA per
-// SM), whatever the batch: a decode step of one long sequence is split over
-// its positions, a batch of prompts over its rows, and no CTA gets more than a
-// unit above the mean.  An item that several CTAs share leaves one partial
-// record (O, m, l of the rows it has) per CTA in the scratch, and the last of
-// them to arrive adds the records in CTA order, so that the result does not
-// depend on who was last.  Every CTA finds its run itself from cu_q and lens.
+// All items' units in a row are cut into one even run per worker, whatever the
+// batch: a decode step of one long sequence is split over its positions, a
+// batch of prompts over its rows, and no worker gets more than a unit above
+// the mean.  Every worker finds its run itself from cu_q and lens.  An item
+// that several workers share leaves one partial record (O, m, l of its rows)
+// per worker in the scratch, and a second launch, whose blocks wait on the
+// SMs for the first to end, adds the records in worker order.
 //
-// A CTA's roles (10 warps):
-//   * warp 8 streams the key tiles: TMA boxes of 64 values x the positions of
-//     a page (or of the tile, if a page is longer), 128-byte swizzle, each lane
-//     one box; a page outside the item's positions is a box past the end of the
-//     pool, which reads zeros;
-//   * warp 9 issues the MMAs: S = Q K^T with Q in TMEM and K (K-major) in shared
-//     memory, O += P V with P in TMEM and V (N-major) in shared memory;
+// A worker is one CTA (one per SM), or with PAIR a cluster of two CTAs that
+// take 128 rows each and share the key tiles: each loads half of K's positions
+// and half of V's columns, and the MMAs of the pair (cta_group::2, M = 256) read
+// both halves.  A single CTA's 128 rows need 64 KB of keys and values per
+// 1024 cycles of tensor work (head_dim 256, 64 positions), which the shared
+// memory cannot take in and hand to the MMAs at that rate; a pair needs half.
+//
+// A CTA's roles (12 warps):
+//   * warp 8 streams the key tiles into a ring of slots, in the order in which
+//     the MMAs use them (K0 K1 V0 K2 V1 ...): TMA boxes of 64 values x the
+//     positions of a page (or of the tile, if a page is longer), 128-byte
+//     swizzle, each lane one box; a page outside the item's positions is a box
+//     past the end of the pool, which reads zeros;
+//   * warp 9 issues the MMAs: S = Q K^T with K (K-major) in shared memory, O += P
+//     V with P in TMEM and V (N-major) in shared memory.  Q is in TMEM, or with
+//     PAIR in shared memory.  In a pair the first CTA's warp issues;
 //   * warps 0-7 have half a row per thread, warps w and w + 4 the halves of the
-//     same rows: Q into TMEM, the softmax of S (the two halves tell each other
-//     their maximum), P back into TMEM, and at the item's end O / l to global
-//     memory.  A warp none of whose rows is live (decode: G rows of 128) only
-//     passes the barriers.
-// TMEM (512 columns): O | Q | S | P, P.  S is free again once the warps
-// have loaded it, so the next product runs while they compute; P has two
-// buffers.  Steady state of the tensor pipe: P V of tile t, Q K of tile t + 2,
-// P V of tile t + 1, ...
+//     same rows: the softmax of S (the two halves tell each other their
+//     maximum), P into TMEM, and at the item's end O / l to global memory.  A
+//     warp none of whose rows is live (decode: G rows of 128) only passes the
+//     barriers.
+// TMEM (512 columns): O | Q | S | P, P (PAIR: O | S | P, P).  S is free again
+// once the warps have loaded it, so the next product runs while they compute;
+// P has two buffers.  Steady state of the tensor pipe: P V of tile t, Q K of
+// tile t + 2, P V of tile t + 1, ...
 //
 // m moves only when the running maximum has grown by more than 2^8 since it
 // was set: weights then stay below 2^8 (fp32 sums, and far from the 16-bit
@@ -43,6 +52,8 @@
 // Rows of a V tile that the item does not see may hold anything: their weights
 // are 0, but 0 * NaN is not, so the softmax warps overwrite them with zeros in
 // shared memory before the product (the first and last tile of an item only).
+//
+// Every wait is bounded (2 s; status 5 and the CTA's abort flag).
 #include <cudaTypedefs.h>
 
 #include "paged_common.cuh"
@@ -59,27 +70,30 @@ struct AttnArgs {
     long long q_stride, out_stride;
     int n_q, window;
     float scale;
-    unsigned *count;  // arrivals at an item, by the CTA that has its first unit
-    float *part;      // two records per CTA
+    struct PaItem *items;  // of each CTA: the item that begins in its run and ends in a later one
+    float *part;           // two records per CTA
     int *status;
+};
+
+// An item whose records are to be joined (np = 0: none).
+struct __align__(16) PaItem {
+    int np, rows, tok, j;  // parts, rows, first token row, kv head
 };
 
 constexpr int PA_ROWS = 128;
 constexpr int PA_SOFTMAX = 8;  // softmax warps: two for each 32 rows, each with half of a tile's positions
 constexpr int PA_PRODUCER = PA_SOFTMAX, PA_ISSUER = PA_SOFTMAX + 1;
 constexpr int PA_THREADS = (PA_SOFTMAX + 2) * 32;
-constexpr int PA_JOIN = 1024;  // (row, part) pairs whose factors are held at once when records are joined
-constexpr int PA_MAX_CTAS = 1024;  // counters in the scratch's first 4096 bytes
-constexpr float PA_SLACK = 8.0f;   // growth of the maximum (log2) before m follows
+constexpr float PA_SLACK = 8.0f;  // growth of the maximum (log2) before m follows
 
 template <int HD> struct PaPlan {
     static constexpr int KT = HD == 256 ? 64 : 128;  // positions per key tile
-    static constexpr int STAGES = HD == 64 ? 6 : 3;
-    static constexpr int TILE = KT * HD * 2;         // bytes of K (or V) of a tile
-    static constexpr int O = 0, Q = HD, S = Q + HD / 2, P = S + KT;  // TMEM columns
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * 2 * TILE + 512;
+    static constexpr int SLOT = KT * HD * 2;         // bytes of a slot (K or V of a tile)
+    static constexpr int SLOTS = 192 * 1024 / SLOT;
+    static constexpr int O = 0, Q = HD, S = HD + HD / 2, P = S + KT;  // TMEM columns: O | Q | S | P, P
+    static constexpr size_t SMEM = 1024 + (size_t)SLOTS * SLOT + 1024;
     static_assert(P + KT <= 512, "TMEM plan");
-    static_assert(SMEM > MMA_SMEM_MIN && SMEM <= MMA_SMEM_LIMIT, "one CTA per SM");
+    static_assert(SMEM > MMA_SMEM_MIN && SMEM <= MMA_SMEM_LIMIT - 8192, "one CTA per SM");
 };
 
 // floats of a partial record: O[d / 4][row][4], then (m, l) of the rows
@@ -87,14 +101,74 @@ __host__ __device__ constexpr size_t pa_record(int hd) { return (size_t)PA_ROWS 
 
 // ---- tensor core helpers ----
 
-// D[tmem] (+)= A[tmem] B[smem], 16-bit operands, fp32 sums, one thread.
-M27B_DI void umma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] B[smem], 16-bit operands, fp32 sums, one thread; for a pair, both CTAs' halves.
+template <bool PAIR>
+M27B_DI void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                     "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                     "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                     : "memory");
+}
+// The same with A in shared memory, for a pair.
+M27B_DI void umma_f16_ss2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// The MMAs that this thread issued for the pair arrive on `bar` of both CTAs when they complete.
+M27B_DI void pair_commit(uint64_t *bar) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
         : "memory");
+}
+M27B_DI void pair_tmem_alloc(uint32_t *slot) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+M27B_DI void pair_tmem_free(uint32_t tmem) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+// All threads of the pair.
+M27B_DI void pair_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The address, in the first or second CTA of the pair, of the barrier at this place.
+M27B_DI uint32_t pair_bar(uint64_t *bar, int cta) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(bar)), "r"(cta));
+    return r;
+}
+// Copies into this CTA that signal a barrier of either CTA of the pair.
+M27B_DI void pair_load_4d(uint32_t dst, const CUtensorMap *tm, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4, %5}], [%6];" ::"r"(dst),
+        "l"((unsigned long long)tm), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+M27B_DI void pair_load_3d(uint32_t dst, const CUtensorMap *tm, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(dst),
+        "l"((unsigned long long)tm), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+// Arrive on the barrier at the same place in the first (or second) CTA of the pair.  What
+// these arrivals announce is in TMEM or was written by copies, whose order the
+// tcgen05 fences and the copies' own barriers give, so they carry no release
+// at cluster scope (some 800 cycles each; zeroed V rows, ordinary stores, get a
+// cluster fence of their own).
+M27B_DI void pair_arrive(uint64_t *bar, int cta = 0) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(pair_bar(bar, cta)) : "memory");
 }
 // Matrix descriptor, 128-byte swizzle: 1024 bytes between groups of 8
 // 128-byte rows; `lead` bytes between 64-value columns (N-major operands).
@@ -102,11 +176,11 @@ M27B_DI uint64_t umma_desc128(uint32_t saddr, uint32_t lead) {
     return (uint64_t)((saddr & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// fp32 accumulator, f16 or bf16 operands, A K-major, B K-major or N-major, M = 128.
-template <bool BF, int N, bool BMN>
+// fp32 accumulator, f16 or bf16 operands, A K-major, B K-major or N-major.
+template <bool BF, int M, int N, bool BMN>
 constexpr uint32_t umma_idesc_f16() {
     return (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((BMN ? 1u : 0u) << 16) |
-           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 M27B_DI void tmem_ld32(uint32_t taddr, uint32_t *v) {
     asm volatile(
@@ -212,11 +286,11 @@ M27B_DI long long pa_head_units(const PaSeq &s, int tq, int window) {
     return u;
 }
 
-// A CTA's run of units, and where it begins.
+// A worker's run of units, and where it begins.
 struct PaRun {
     long long total, begin, end;
-    int ctas;             // CTAs that have a run
-    int b, j, r, off;     // first item, and units of it that belong to the CTAs before
+    int workers;          // workers that have a run
+    int b, j, r, off;     // first item, and units of it that belong to the workers before
     long long seq_off, head_units;  // the run's begin within sequence b; units of a kv head of it
     PaSeq seq;                      // sequence b
 };
@@ -284,7 +358,7 @@ M27B_DI long long pa_scan(long long v, long long *red, long long *total) {
     if (lane == 31) red[warp] = inc;
     __syncthreads();
     long long before = 0, all = 0;
-    for (int w = 0; w < PA_THREADS / 32; ++w) {
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
         if (w < warp) before += red[w];
         all += red[w];
     }
@@ -292,13 +366,13 @@ M27B_DI long long pa_scan(long long v, long long *red, long long *total) {
     return before + inc - v;
 }
 
-// All threads: fill `run` (shared memory) with this CTA's run.
+// All threads: fill `run` (shared memory) with the run of worker `me` of at most `most`.
 template <int KT>
-M27B_DI void pa_find_run(const AttnArgs &a, int tq, PaRun *run, long long *red) {
-    const int n = a.bt.n_seq;
+M27B_DI void pa_find_run(const AttnArgs &a, int tq, int me, int most, PaRun *run, long long *red) {
+    const int n = a.bt.n_seq, nt = blockDim.x;
     long long total = 0, head = 0, u = 0, before = 0, sum;
     PaSeq s;
-    for (int b0 = 0; b0 < n; b0 += PA_THREADS) {
+    for (int b0 = 0; b0 < n; b0 += nt) {
         const int b = b0 + threadIdx.x;
         s = {0, 0, 0, 0, 0};
         if (b < n) s = pa_seq(a, b, tq, blockIdx.x == 0);
@@ -307,19 +381,19 @@ M27B_DI void pa_find_run(const AttnArgs &a, int tq, PaRun *run, long long *red) 
         before = pa_scan(u, red, &sum);
         total += sum;
     }
-    const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
-    const long long begin = c < ctas ? div_count(c * total, ctas) : 0,
-                    end = c < ctas ? div_count((c + 1) * total, ctas) : 0;
+    const long long n_w = min((long long)most, total);
+    const long long begin = me < n_w ? div_count(me * total, n_w) : 0,
+                    end = me < n_w ? div_count((me + 1) * total, n_w) : 0;
     if (threadIdx.x == 0) {
-        run->total = total, run->ctas = (int)ctas, run->begin = begin, run->end = end;
+        run->total = total, run->workers = (int)n_w, run->begin = begin, run->end = end;
         run->b = n;
     }
     __syncthreads();
     if (begin >= end) return;
     long long at = 0;
-    for (int b0 = 0; b0 < n && at <= begin; b0 += PA_THREADS) {
+    for (int b0 = 0; b0 < n && at <= begin; b0 += nt) {
         const int b = b0 + threadIdx.x;
-        if (n > PA_THREADS) {
+        if (n > nt) {
             s = {0, 0, 0, 0, 0};
             if (b < n) s = pa_seq(a, b, tq, false);
             head = pa_head_units<KT>(s, tq, a.window);
@@ -366,215 +440,228 @@ struct PaShared {
     PaRun run;
     long long red[PA_THREADS / 32];
     float half[2][2][PA_ROWS];  // what the two warps of a row tell each other, by turns
-    float2 join[PA_JOIN];
     uint32_t tmem;
     int abort;
-    int last;
 };
 
-// Add up the np records of an item of CTAs c0, c0 + 1, ... and write its rows;
-// the softmax warps of the CTA that arrived last.  Rows are taken so many at a
-// time that their parts' m and l fit `join`, fetched in one round trip; a
-// part's factor is 2^(m - max) / sum.  Then four quadruples of values x four
-// parts a thread are in flight.
-template <int HD, bool BF, class Walk, class Sync>
-M27B_DI bool pa_join(const AttnArgs &a, const Walk &w, int c0, int np, int rows, int G, int tq, float2 *join, int tid,
-                     Sync all_here) {
-    constexpr int NT = 32 * PA_SOFTMAX;
-    auto record = [&](int x) { return a.part + (size_t)(2 * (c0 + x) + (x == 0 ? 1 : 0)) * pa_record(HD); };
-    const int at_once = min(rows, PA_JOIN / np);
-    for (int r0 = 0; r0 < rows; r0 += at_once) {
-        const int nr = min(at_once, rows - r0);
-        for (int e = tid; e < nr * np; e += NT) {
-            const int x = e / nr;
-            join[e] = __ldcg((const float2 *)(record(x) + (size_t)PA_ROWS * HD) + r0 + e - x * nr);
-        }
-        if (!all_here()) return false;
-        for (int r = tid; r < nr; r += NT) {
-            float mx = -INFINITY, ls = 0.0f;
-            for (int x = 0; x < np; ++x) mx = fmaxf(mx, join[x * nr + r].x);
-            const float ref = mx == -INFINITY ? 0.0f : mx;
-            for (int x = 0; x < np; ++x) {
-                const float2 ml = join[x * nr + r];
-                const float f = ex2(ml.x - ref);
-                join[x * nr + r].x = f;
-                ls = fmaf(f, ml.y, ls);
-            }
-            const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
-            for (int x = 0; x < np; ++x) join[x * nr + r].x *= inv;
-            if (a.lse)
-                a.lse[(w.s.q_lo + w.r * tq + (r0 + r) / G) * (long long)a.n_q + w.j * G + (r0 + r) % G] =
-                    ls > 0.0f ? 0.69314718055994530942f * (mx + log2f(ls)) : -INFINITY;
-        }
-        if (!all_here()) return false;
-        for (int e0 = tid; e0 < nr * (HD / 4); e0 += 4 * NT) {
-            float4 o[4] = {};
-            int rr[4], dd[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) dd[g] = (e0 + NT * g) / nr, rr[g] = e0 + NT * g - dd[g] * nr;
-            for (int x0 = 0; x0 < np; x0 += 4) {
-                float4 y[4][4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const float4 *rx = (const float4 *)record(x0 + x) + r0;
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        y[g][x] = x0 + x < np && dd[g] < HD / 4 ? __ldcg(rx + (size_t)dd[g] * PA_ROWS + rr[g])
-                                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const float f = x0 + x < np ? join[(x0 + x) * nr + rr[g]].x : 0.0f;
-                        o[g].x = fmaf(f, y[g][x].x, o[g].x), o[g].y = fmaf(f, y[g][x].y, o[g].y);
-                        o[g].z = fmaf(f, y[g][x].z, o[g].z), o[g].w = fmaf(f, y[g][x].w, o[g].w);
-                    }
-            }
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                if (dd[g] >= HD / 4) continue;
-                const long long tk = w.s.q_lo + w.r * tq + (r0 + rr[g]) / G;
-                *(uint2 *)((uint16_t *)a.out + tk * a.out_stride + (long long)(w.j * G + (r0 + rr[g]) % G) * HD + 4 * dd[g]) =
-                    make_uint2(Half16<BF>::down(o[g].x, o[g].y), Half16<BF>::down(o[g].z, o[g].w));
-            }
-        }
-        if (r0 + at_once < rows && !all_here()) return false;  // the factors are about to be replaced
-    }
+// Page id of page p of the sequence for a copy: past the end of the pool (a box
+// of zeros) where the item sees nothing of the page.
+template <class Walk>
+M27B_DI int pa_page(const AttnArgs &a, const Walk &w, const int *ids, int p, int shift) {
+    if (p >= a.kv.n_cols || (p << shift) >= w.sp.hi || (p + 1) << shift <= w.sp.lo) return a.kv.n_pages;
+    const int id = __ldg(ids + p);
+    if (id >= 0 && id < a.kv.n_pages) return id;
+    paged_bad(a.status);
+    return a.kv.n_pages;
+}
+
+// Bounded waits.  The timer and the abort flag are looked at only after many
+// tests (a test may itself wait a while in hardware), out of line: what stands
+// between the roles' hand-offs is a test and a branch.
+__device__ __noinline__ bool pa_give_up(unsigned long long &t0, volatile int *abort, int *status) {
+    if (*abort) return true;
+    const unsigned long long now = global_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 <= M27B_WAIT_NS) return false;
+    *abort = 1;
+    if (status) atomicCAS(status, 0, 5);
     return true;
+}
+M27B_DI bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    unsigned long long t0 = 0;
+    for (unsigned it = 1; !mbar_try_wait(bar, parity); ++it)
+        if ((it & 63u) == 0 && pa_give_up(t0, abort, status)) return false;
+    return true;
+}
+M27B_DI bool pa_warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, status)) != 0;
+}
+
+// The end of an item in this worker's run: this thread's half of its row's O
+// (columns [half HD / 2, ..) of TMEM at `o`) to the output, or, if the worker
+// has a part of the item only, O, m and l to its record.  `tok`: the first
+// token row of the CTA's rows; `any`: there were tiles (else O is 0).
+template <int HD, bool BF, class Walk>
+M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me, int cta, int tok, int G, int rows, int row,
+                      int half, bool any, float m, float l, uint32_t o, PaItem &tail) {
+    const bool live = row < rows, idle = (row & ~31) >= rows;
+    const int h = w.j * G + row % G;
+    const long long at = tok + row / G;
+    if (w.whole()) {
+        if (idle) return;
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint16_t *op = (uint16_t *)a.out + at * a.out_stride + (long long)h * HD + half * (HD / 2);
+#pragma unroll 1
+        for (int x = 0; x < HD / 64; ++x) {
+            uint32_t v[32];
+            if (any) {
+                tmem_ld32(o + half * (HD / 2) + 32 * x, v);
+                tmem_wait_ld();
+            }
+            if (live)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        y[d] = l > 0.0f ? Half16<BF>::down(__uint_as_float(v[8 * e + 2 * d]) * inv,
+                                                           __uint_as_float(v[8 * e + 2 * d + 1]) * inv)
+                                        : 0u;
+                    *((uint4 *)(op + 32 * x) + e) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+        }
+        if (live && a.lse && half == 0)
+            a.lse[at * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
+    } else {
+        // the item begins with worker c0 and ends with c1
+        const long long U = w.u - w.off;
+        const int c0 = (int)div_count((U + 1) * run.workers + run.total - 1, run.total) - 1;
+        const int c1 = (int)div_count((U + w.sp.units()) * run.workers + run.total - 1, run.total) - 1;
+        if (me == c0) tail = {rows > 0 ? c1 - c0 + 1 : 0, rows, tok, w.j};
+        if (idle) return;
+        float *rec = a.part + (size_t)(2 * cta + (me == c0 ? 1 : 0)) * pa_record(HD);
+#pragma unroll 1
+        for (int x = 0; x < HD / 64; ++x) {
+            uint32_t v[32];
+            tmem_ld32(o + half * (HD / 2) + 32 * x, v);
+            tmem_wait_ld();
+            if (live)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    __stcg((uint4 *)rec + (size_t)(half * (HD / 8) + 8 * x + e) * PA_ROWS + row,
+                           make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
+        }
+        if (live && half == 0) __stcg((float2 *)(rec + (size_t)PA_ROWS * HD) + row, make_float2(m, l));
+    }
+    tc_fence_before();
 }
 
 template <int HD, bool BF>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     k_paged_attn(const AttnArgs a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
     using L = PaPlan<HD>;
-    constexpr int KT = L::KT, ST = L::STAGES, TILE = L::TILE, NCH = HD / 64;
+    constexpr int KT = L::KT, NS = L::SLOTS, SLOT = L::SLOT;
     extern __shared__ uint8_t pa_raw[];
-    uint8_t *smem = (uint8_t *)(((uintptr_t)pa_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = (uint64_t *)(smem + (size_t)ST * 2 * TILE);
-    uint64_t *kfull = bars, *vfull = kfull + ST, *empty = vfull + ST, *qfull = empty + ST, *sfull = qfull + 1,
-             *sfree = sfull + 1, *pfull = sfree + 1, *pdone = pfull + 2, *drain = pdone + 2, *meet = drain + 1, *pair = meet + 1;
+    uint8_t *ring = (uint8_t *)(((uintptr_t)pa_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = (uint64_t *)(ring + (size_t)NS * SLOT);
+    // full: a slot's copies have landed; empty: its MMAs are done
+    uint64_t *full = bars, *empty = full + NS, *qfull = empty + NS, *sfull = qfull + 1, *sfree = sfull + 1,
+             *pfull = sfree + 1, *pdone = pfull + 2, *drain = pdone + 2, *pair = drain + 1;
     __shared__ PaShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = a.n_q / a.kv.n_kv, tq = PA_ROWS / G;
+    const int me = blockIdx.x, G = a.n_q / a.kv.n_kv, tq = PA_ROWS / G;  // tokens of an item
     volatile int *abort = &sh.abort;
 
-    if (tid == 0) {
-        for (int s = 0; s < ST; ++s) {
-            mbar_init(&kfull[s], 1);
-            mbar_init(&vfull[s], 1);
-            mbar_init(&empty[s], 1);
+    if (warp == PA_PRODUCER) {
+        for (int s = lane; s < 2 * NS; s += 32) mbar_init(&full[s], 1);
+        if (lane < 4) mbar_init(&pair[lane], 2);
+        if (lane < 2) {
+            mbar_init(&pfull[lane], PA_SOFTMAX);
+            mbar_init(&pdone[lane], 1);
         }
-        mbar_init(qfull, PA_SOFTMAX);
-        mbar_init(sfull, 1);
-        mbar_init(sfree, PA_SOFTMAX);
-        for (int i = 0; i < 4; ++i) mbar_init(&pair[i], 2);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&pfull[i], PA_SOFTMAX);
-            mbar_init(&pdone[i], 1);
+        if (lane == 0) {
+            mbar_init(qfull, PA_SOFTMAX);
+            mbar_init(sfull, 1);
+            mbar_init(sfree, PA_SOFTMAX);
+            mbar_init(drain, 1);
+            sh.abort = 0;
         }
-        mbar_init(drain, 1);
-        mbar_init(meet, PA_SOFTMAX);
-        sh.abort = 0;
         fence_mbar_init();
     }
-    if (warp == 0) {
+    if (warp == PA_ISSUER) {
         tmem_alloc(&sh.tmem, 512);
         tmem_relinquish();
     }
     pdl_wait();
     pdl_trigger();
     tc_fence_before();
-    pa_find_run<KT>(a, tq, &sh.run, sh.red);
+    pa_find_run<KT>(a, tq, me, gridDim.x, &sh.run, sh.red);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     PaWalk<KT> w(a, sh.run, tq);
 
     if (warp == PA_PRODUCER) {
-        // lane = box: K or V, 64-value column, page of the tile
-        const int ps = a.kv.page_size, rows = min(ps, KT), npp = KT / rows;
-        const int pg = lane % npp, ch = (lane / npp) % NCH, isv = lane / (npp * NCH);
-        const uint32_t dst0 = smem_u32(smem) + isv * TILE + ch * (KT * 128) + pg * rows * 128;
-        const int shift = 31 - __clz(ps);
-        int t = 0;
+        const int ps = a.kv.page_size, shift = 31 - __clz(ps);
+        // lane = box: (64-value column, page of the tile)
+        const int rows = min(ps, KT), np = KT / rows, pg = lane % np, ch = lane / np;
+        const uint32_t base = smem_u32(ring);
+        const uint32_t dst = ch * (KT * 128) + pg * rows * 128;
+        int g = 0;
         bool ok = true;
         for (; ok && w.more(); w.next()) {
             const int n = w.tiles();
+            if (n == 0) continue;
             const int *ids = a.kv.table + (long long)w.s.row * a.kv.n_cols;
-            int have = -1, cur = 0;  // lane's page id of pages have + lane
-            for (int i = 0; i < n; ++i, ++t) {
-                const int s = t % ST, x0 = (w.first() + i) * KT, p0 = x0 >> shift;
-                if (have < 0 || p0 < have || p0 + npp > have + 32) {
-                    have = p0;
-                    const int p = have + lane;
-                    const bool in = p < a.kv.n_cols && (p << shift) < w.sp.hi && (p + 1) << shift > w.sp.lo;
-                    cur = in ? __ldg(ids + p) : a.kv.n_pages;
-                    if (cur < 0 || cur > a.kv.n_pages || (in && cur == a.kv.n_pages)) {
-                        paged_bad(a.status);
-                        cur = a.kv.n_pages;
+            int have = -32, cur = 0;  // lane's page id of page have + lane of the sequence
+            // page ids of the tile at x0 (and, in the same fetch, of the one before: its V comes after this K)
+            auto page_of = [&](int p) { return __shfl_sync(0xffffffffu, cur, (p - have) & 31); };
+            for (int i = 0; ok && i <= n; ++i) {
+                if (i < n) {
+                    const int x0 = (w.first() + i) * KT, plast = (x0 + KT - 1) >> shift;
+                    if (plast >= have + 32) {
+                        have = max(0, x0 - KT) >> shift;
+                        cur = pa_page(a, w, ids, have + lane, shift);
                     }
+                    const int s = g % NS, page = page_of((x0 >> shift) + pg);
+                    if (g >= NS && !(ok = pa_warp_wait(&empty[s], (uint32_t)((g / NS - 1) & 1), abort, a.status))) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], SLOT);
+                    __syncwarp();
+                    if (ch < HD / 64) tma_load_4d(base + s * SLOT + dst, &tmk, ch * 64, x0 & (ps - 1), w.j, page, &full[s]);
+                    ++g;
                 }
-                const int page = __shfl_sync(0xffffffffu, cur, p0 + pg - have);
-                if (t >= ST && !warp_wait_or_abort(&empty[s], (uint32_t)((t / ST - 1) & 1), abort, a.status)) {
-                    ok = false;
-                    break;
+                if (i > 0) {
+                    const int x0 = (w.first() + i - 1) * KT, s = g % NS, page = page_of((x0 >> shift) + pg);
+                    if (g >= NS && !(ok = pa_warp_wait(&empty[s], (uint32_t)((g / NS - 1) & 1), abort, a.status))) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], SLOT);
+                    __syncwarp();
+                    if (ch < HD / 64) tma_load_4d(base + s * SLOT + dst, &tmv, ch * 64, x0 & (ps - 1), w.j, page, &full[s]);
+                    ++g;
                 }
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&kfull[s], TILE);
-                    mbar_arrive_expect_tx(&vfull[s], TILE);
-                }
-                __syncwarp();
-                if (isv < 2)
-                    tma_load_4d(dst0 + s * 2 * TILE, isv ? &tmv : &tmk, ch * 64, x0 & (ps - 1), w.j,
-                                page, isv ? &vfull[s] : &kfull[s]);
             }
         }
         // every copy lands before the CTA's shared memory is released (bounded)
-        for (int i = max(0, t - ST); i < t; ++i) {
-            mbar_wait_bounded(&kfull[i % ST], (uint32_t)((i / ST) & 1), a.status, 5);
-            mbar_wait_bounded(&vfull[i % ST], (uint32_t)((i / ST) & 1), a.status, 5);
-        }
+        for (int i = max(0, g - NS); i < g; ++i) mbar_wait_bounded(&full[i % NS], (uint32_t)((i / NS) & 1), a.status, 5);
     } else if (warp == PA_ISSUER) {
         if (lane == 0) {
-            constexpr uint32_t id_s = umma_idesc_f16<BF, KT, false>(), id_o = umma_idesc_f16<BF, HD, true>();
-            const uint32_t base = smem_u32(smem);
-            int t0 = 0, item = 0;
+            constexpr uint32_t id_s = umma_idesc_f16<BF, 128, KT, false>(), id_o = umma_idesc_f16<BF, 128, HD, true>();
+            const uint32_t base = smem_u32(ring);
+            int t0 = 0, g = 0, item = 0;
             bool ok = true;
+            auto landed = [&](int g) { return pa_wait(&full[g % NS], (uint32_t)((g / NS) & 1), abort, a.status); };
             for (; ok && w.more(); w.next()) {
                 const int n = w.tiles();
                 if (n == 0) continue;
                 // S of tile t = Q K^T, once S has been read and the keys are there
                 auto scores = [&](int t) {
-                    if (t > 0 && !wait_or_abort(sfree, (uint32_t)((t - 1) & 1), abort, a.status)) return false;
-                    if (!wait_or_abort(&kfull[t % ST], (uint32_t)((t / ST) & 1), abort, a.status)) return false;
+                    if (t > 0 && !pa_wait(sfree, (uint32_t)((t - 1) & 1), abort, a.status)) return false;
+                    if (!landed(g)) return false;
                     tc_fence_after();
-                    const uint32_t k = base + (t % ST) * 2 * TILE;
+                    const uint32_t k = base + (g % NS) * SLOT;
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk)
-                        umma_f16_ts(tmem + L::S, tmem + L::Q + kk * 8,
-                                    umma_desc128(k + (kk / 4) * (KT * 128) + (kk % 4) * 32, 16), id_s, kk > 0);
+                        umma_f16_ts<false>(tmem + L::S, tmem + L::Q + kk * 8,
+                                           umma_desc128(k + (kk / 4) * (KT * 128) + (kk % 4) * 32, 16), id_s, kk > 0);
                     umma_commit(sfull);
+                    umma_commit(&empty[g % NS]);
+                    ++g;
                     return true;
                 };
-                ok = wait_or_abort(qfull, (uint32_t)(item & 1), abort, a.status);
+                ok = pa_wait(qfull, (uint32_t)(item & 1), abort, a.status);
                 tc_fence_after();
                 ok = ok && scores(t0) && (n < 2 || scores(t0 + 1));
                 for (int i = 0; ok && i < n; ++i) {
                     const int t = t0 + i;
-                    if (!wait_or_abort(&pfull[t & 1], (uint32_t)((t >> 1) & 1), abort, a.status) ||
-                        !wait_or_abort(&vfull[t % ST], (uint32_t)((t / ST) & 1), abort, a.status)) {
-                        ok = false;
-                        break;
-                    }
+                    if (!(ok = pa_wait(&pfull[t & 1], (uint32_t)((t >> 1) & 1), abort, a.status) && landed(g))) break;
                     tc_fence_after();
-                    const uint32_t v = base + (t % ST) * 2 * TILE + TILE;
+                    const uint32_t v = base + (g % NS) * SLOT;
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
-                        umma_f16_ts(tmem + L::O, tmem + L::P + (t & 1) * (KT / 2) + kk * 8,
-                                    umma_desc128(v + kk * 2048, KT * 128), id_o, i > 0 || kk > 0);
-                    umma_commit(&empty[t % ST]);
+                        umma_f16_ts<false>(tmem + L::O, tmem + L::P + (t & 1) * (KT / 2) + kk * 8,
+                                           umma_desc128(v + kk * 2048, KT * 128), id_o, i > 0 || kk > 0);
+                    umma_commit(&empty[g % NS]);
                     umma_commit(&pdone[t & 1]);
+                    ++g;
                     if (i + 2 < n) ok = scores(t + 2);
                 }
                 t0 += n;
@@ -592,27 +679,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int quarter = warp & 3, half = warp >> 2, row = 32 * quarter + lane;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
         const float c = a.scale * 1.44269504088896340736f;  // log2 e
-        int t = 0, met = 0, told = 0;
+        int t = 0, g0 = 0, told = 0;
         bool ok = true;
-        // the softmax warps wait for one another (bounded: a warp that gave up never comes)
-        auto all_here = [&] {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(meet);
-            return warp_wait_or_abort(meet, (uint32_t)(met++ & 1), abort, a.status);
-        };
+        PaItem tail = {0, 0, 0, 0};
         // this row's value of the other half
         auto other = [&](float mine, float &theirs) {
             const int turn = told++ & 1;
             sh.half[turn][half][row] = mine;
             __syncwarp();
             if (lane == 0) mbar_arrive(&pair[quarter]);
-            const bool here = warp_wait_or_abort(&pair[quarter], (uint32_t)turn, abort, a.status);
+            const bool here = pa_warp_wait(&pair[quarter], (uint32_t)turn, abort, a.status);
             theirs = *(volatile float *)&sh.half[turn][half ^ 1][row];
             return here;
         };
         for (; ok && w.more(); w.next()) {
-            const int n = w.tiles(), i = w.r * tq + row / G, h = w.j * G + row % G;
-            const int rows = min(tq, w.s.q_n - w.r * tq) * G;
+            const int n = w.tiles(), i0 = w.r * tq, i = i0 + row / G, h = w.j * G + row % G;
+            const int rows = min(tq, w.s.q_n - i0) * G;
             const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
             // a dead row's scores are garbage that no one reads
             const int hi = live ? w.s.base + i + 1 : 0x7fffffff;
@@ -638,7 +720,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             for (int k = 0; k < n; ++k, ++t) {
                 const int x0 = (w.first() + k) * KT;
-                if (!(ok = warp_wait_or_abort(sfull, (uint32_t)(t & 1), abort, a.status))) break;
+                if (!(ok = pa_warp_wait(sfull, (uint32_t)(t & 1), abort, a.status))) break;
                 if (idle) {
                     if (lane == 0) mbar_arrive(sfree);
                 } else {
@@ -669,7 +751,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         l *= f;
                         if (k > 0) {
                             // this half's columns of O, once the products so far are done
-                            if (!(ok = warp_wait_or_abort(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status)))
+                            if (!(ok = pa_warp_wait(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status)))
                                 break;
                             tc_fence_after();
 #pragma unroll 1
@@ -695,16 +777,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     // P's buffer is free once the product of two tiles ago is done
-                    if (t >= 2 && !(ok = warp_wait_or_abort(&pdone[t & 1], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status))) break;
+                    if (t >= 2 && !(ok = pa_warp_wait(&pdone[t & 1], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status))) break;
                     const uint32_t pc = lane_base + L::P + (t & 1) * (KT / 2) + half * (KH / 2);
                     if constexpr (KH == 64) tmem_st32(pc, p);
                     else tmem_st16(pc, p);
                 }
                 // values of positions that no row of the item sees
                 if (x0 < w.sp.lo || x0 + KT > w.sp.hi) {
-                    if (!(ok = warp_wait_or_abort(&vfull[t % ST], (uint32_t)((t / ST) & 1), abort, a.status))) break;
-                    uint8_t *v = smem + (size_t)(t % ST) * 2 * TILE + TILE;
-                    for (int e = tid; e < KT * NCH * 8; e += 32 * PA_SOFTMAX) {
+                    const int g = g0 + (k == n - 1 ? 2 * n - 1 : 2 * k + 2);  // V's slot: K0 K1 V0 K2 V1 ...
+                    if (!(ok = pa_warp_wait(&full[g % NS], (uint32_t)((g / NS) & 1), abort, a.status))) break;
+                    uint8_t *v = ring + (size_t)(g % NS) * SLOT;
+                    for (int e = tid; e < SLOT / 16; e += 32 * PA_SOFTMAX) {
                         const int x = (e >> 3) % KT;
                         if (x0 + x < w.sp.lo || x0 + x >= w.sp.hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
                     }
@@ -716,8 +799,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 if (lane == 0) mbar_arrive(&pfull[t & 1]);
             }
             if (!ok) break;
+            g0 += 2 * n;
             if (n > 0) {
-                if (!(ok = warp_wait_or_abort(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status))) break;
+                if (!(ok = pa_warp_wait(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status))) break;
                 tc_fence_after();
             }
             if (!idle) {
@@ -725,71 +809,509 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 if (!(ok = other(l, theirs))) break;
                 l = half ? theirs + l : l + theirs;
             }
-            const long long tok = w.s.q_lo + i;
-            if (w.whole()) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                uint16_t *op = (uint16_t *)a.out + tok * a.out_stride + (long long)h * HD + half * (HD / 2);
-#pragma unroll 1
-                for (int x = 0; x < (idle ? 0 : HD / 64); ++x) {
-                    uint32_t v[32];
-                    if (n > 0) {
-                        tmem_ld32(lane_base + L::O + half * (HD / 2) + 32 * x, v);
-                        tmem_wait_ld();
-                    }
-                    if (live)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint32_t y[4];
-#pragma unroll
-                            for (int d = 0; d < 4; ++d)
-                                y[d] = l > 0.0f ? Half16<BF>::down(__uint_as_float(v[8 * e + 2 * d]) * inv,
-                                                                   __uint_as_float(v[8 * e + 2 * d + 1]) * inv)
-                                                : 0u;
-                            *((uint4 *)(op + 32 * x) + e) = make_uint4(y[0], y[1], y[2], y[3]);
-                        }
-                }
-                if (live && a.lse && half == 0)
-                    a.lse[tok * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
-                tc_fence_before();
-            } else {
-                // this CTA's part of the item; the last of the item's CTAs adds them up
-                const long long U = w.u - w.off;
-                const int c0 = (int)div_count((U + 1) * sh.run.ctas + sh.run.total - 1, sh.run.total) - 1;
-                const int c1 = (int)div_count((U + w.sp.units()) * sh.run.ctas + sh.run.total - 1, sh.run.total) - 1;
-                const int me = blockIdx.x;
-                float *rec = a.part + (size_t)(2 * me + (me == c0 ? 1 : 0)) * pa_record(HD);
-#pragma unroll 1
-                for (int x = 0; x < (idle ? 0 : HD / 64); ++x) {
-                    uint32_t v[32];
-                    tmem_ld32(lane_base + L::O + half * (HD / 2) + 32 * x, v);
-                    tmem_wait_ld();
-                    if (live)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            __stcg((uint4 *)rec + (size_t)(half * (HD / 8) + 8 * x + e) * PA_ROWS + row,
-                                   make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
-                }
-                if (live && half == 0) __stcg((float2 *)(rec + (size_t)PA_ROWS * HD) + row, make_float2(m, l));
-                tc_fence_before();
-                __threadfence();
-                if (!(ok = all_here())) break;
-                if (tid == 0) {
-                    const bool last = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
-                    if (last) a.count[c0] = 0u;
-                    __threadfence();
-                    sh.last = last;
-                }
-                if (!(ok = all_here())) break;
-                if (*(volatile int *)&sh.last) ok = pa_join<HD, BF>(a, w, c0, c1 - c0 + 1, rows, G, tq, sh.join, tid, all_here);
-            }
+            pa_write<HD, BF>(a, w, sh.run, me, blockIdx.x, w.s.q_lo + i0, G, rows, row, half, n > 0, m, l, lane_base + L::O, tail);
         }
+        if (tid == 0) a.items[blockIdx.x] = tail;
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == PA_ISSUER) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+}
+
+// ---- two CTAs a worker ----
+
+template <int HD> struct PairPlan {
+    static constexpr int KT = 128;                   // positions per key tile
+    static constexpr int KR = KT / 2, VC = HD / 2;   // positions of K, columns of V in a CTA's slot
+    static constexpr int SLOT = KR * HD * 2;
+    static_assert(SLOT == KT * VC * 2, "slots");
+    static constexpr int Q_BYTES = PA_ROWS * HD * 2;
+    static constexpr int SLOTS = (192 * 1024 - Q_BYTES) / SLOT;
+    static constexpr int NB = HD == 256 ? 1 : 2;     // buffers of S
+    static constexpr int O = 0, S = HD, P = S + NB * KT;  // TMEM columns: O | S (, S) | P, P
+    static constexpr size_t SMEM = 1024 + Q_BYTES + (size_t)SLOTS * SLOT + 1024;
+    static_assert(P + KT <= 512, "TMEM plan");
+    static_assert(SMEM > MMA_SMEM_MIN && SMEM <= MMA_SMEM_LIMIT - 8192, "one CTA per SM");
+};
+// Registers: the softmax warps hold a row of a tile; 2 x 128 threads of 216 and
+// 128 of 72 are the 384 x 168 that the block is launched with.
+constexpr int PAIR_THREADS = (PA_SOFTMAX + 4) * 32;
+constexpr int PAIR_REGS_SOFTMAX = 216, PAIR_REGS_OTHER = 72;
+static_assert(2 * PAIR_REGS_SOFTMAX + PAIR_REGS_OTHER <= 3 * 168, "register split");
+
+struct PairShared {
+    PaRun run;
+    long long red[PAIR_THREADS / 32];
+    uint2 m[2][PA_ROWS];        // a row's m after a tile, by turns, with the tile's number + 1
+    float half[2][2][PA_ROWS];  // what the two warps of a row tell each other at an item's end
+    uint32_t tmem;
+    int abort;
+};
+
+// Two values at once (packed fp32 arithmetic).
+M27B_DI uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+M27B_DI float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+M27B_DI uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+M27B_DI uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+M27B_DI float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// The m that another warp stores with number `tag` (bounded, for a whole warp).
+M27B_DI bool pair_follow(const uint2 *p, uint32_t tag, float &m, volatile int *abort, int *status) {
+    uint2 v;
+    const uint32_t at = smem_u32(p);
+    unsigned long long t0 = 0;
+    bool here = true;
+    for (unsigned it = 1;; ++it) {
+        asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+        if (v.y == tag) break;
+        if ((it & 255u) == 0 && pa_give_up(t0, abort, status)) {
+            here = false;
+            break;
+        }
+    }
+    m = __uint_as_float(v.x);
+    return __all_sync(0xffffffffu, here) != 0;
+}
+
+template <int HD, bool BF>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    k_paged_attn_pair(const AttnArgs a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                      const __grid_constant__ CUtensorMap tmq) {
+    using L = PairPlan<HD>;
+    constexpr int KT = L::KT, NS = L::SLOTS, SLOT = L::SLOT, NB = L::NB, WARPS = 2 * PA_SOFTMAX;
+    extern __shared__ uint8_t pa_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)pa_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *ring = smem + L::Q_BYTES;
+    uint64_t *bars = (uint64_t *)(ring + (size_t)NS * SLOT);
+    // full: a slot's copies have landed (in the first CTA, for those of both);
+    // empty: its MMAs are done; sfull, pdone, empty, qempty come to both CTAs;
+    // sfree, pfull, oread are the first CTA's, for the warps of both; vlanded tells
+    // the second CTA's softmax warps that a tile's V is there
+    uint64_t *full = bars, *empty = full + NS, *qfull = empty + NS, *qempty = qfull + 1, *vlanded = qempty + 1, *sfull = vlanded + 2, *sfree = sfull + 2, *pfull = sfree + 2, *pdone = pfull + 2,
+             *oread = pdone + 2, *drain = oread + 1, *pair = drain + 1;
+    __shared__ PairShared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x & 1, me = blockIdx.x >> 1;
+    const int G = a.n_q / a.kv.n_kv, tq = PA_ROWS / G, tqw = 2 * tq;  // tokens of a CTA's rows, of an item
+    volatile int *abort = &sh.abort;
+
+    if (warp == PA_PRODUCER) {
+        for (int s = lane; s < 2 * NS; s += 32) mbar_init(&full[s], 1);
+        if (lane < 4) mbar_init(&pair[lane], 2);
+        if (lane < 2) {
+            mbar_init(&sfull[lane], 1);
+            mbar_init(&vlanded[lane], 1);
+            mbar_init(&sfree[lane], WARPS / 2);
+            mbar_init(&pfull[lane], WARPS / 2);
+            mbar_init(&pdone[lane], 1);
+        }
+        if (lane == 0) {
+            mbar_init(qfull, 1);
+            mbar_init(qempty, 1);
+            mbar_init(oread, WARPS);
+            mbar_init(drain, 1);
+            sh.abort = 0;
+        }
+        fence_mbar_init();
+    }
+    if (warp == PA_ISSUER) pair_tmem_alloc(&sh.tmem);
+    if (tid < 2 * PA_ROWS) sh.m[tid >> 7][tid & 127].y = 0;
+    pdl_wait();
+    pdl_trigger();
+    tc_fence_before();
+    pa_find_run<KT>(a, tqw, me, gridDim.x >> 1, &sh.run, sh.red);
+    pair_barrier();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    PaWalk<KT> w(a, sh.run, tqw);
+    auto fewer_registers = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_OTHER)); };
+
+    if (warp == PA_PRODUCER) {
+        fewer_registers();
+        const int ps = a.kv.page_size, shift = 31 - __clz(ps);
+        // lane = box: (64-value column, page) of a K slot or a V slot
+        const int krows = min(ps, L::KR), knp = L::KR / krows, vrows = min(ps, KT), vnp = KT / vrows;
+        const int kpg = lane % knp, kch = lane / knp, vpg = lane % vnp, vch = lane / vnp;
+        const uint32_t base = smem_u32(ring);
+        const uint32_t kdst = kch * (L::KR * 128) + kpg * krows * 128, vdst = vch * (KT * 128) + vpg * vrows * 128;
+        int g = 0, item = 0;
+        bool ok = true;
+        for (; ok && w.more(); w.next()) {
+            const int n = w.tiles();
+            if (n == 0) continue;
+            if (item > 0 && !(ok = pa_warp_wait(qempty, (uint32_t)((item - 1) & 1), abort, a.status))) break;
+            if (lane == 0 && rank == 0) mbar_arrive_expect_tx(qfull, 2 * (HD / 64) * G * tq * 128);
+            if (lane < HD / 64)
+                pair_load_3d(smem_u32(smem) + lane * (PA_ROWS * 128), &tmq, lane * 64, w.j * G,
+                             w.s.q_lo + w.r * tqw + rank * tq, pair_bar(qfull, 0));
+            ++item;
+            const int *ids = a.kv.table + (long long)w.s.row * a.kv.n_cols;
+            int have = -32, cur = 0;  // lane's page id of page have + lane of the sequence
+            auto page_of = [&](int p) { return __shfl_sync(0xffffffffu, cur, (p - have) & 31); };
+            for (int i = 0; ok && i < n + NB; ++i) {
+                if (i < n) {
+                    const int x0 = (w.first() + i) * KT, plast = (x0 + KT - 1) >> shift;
+                    if (plast >= have + 32) {
+                        // from NB tiles before on: that V comes after this K
+                        have = max(0, x0 - NB * KT) >> shift;
+                        cur = pa_page(a, w, ids, have + lane, shift);
+                    }
+                    const int s = g % NS, xk = x0 + rank * L::KR, page = page_of((xk >> shift) + kpg);
+                    if (g >= NS && !(ok = pa_warp_wait(&empty[s], (uint32_t)((g / NS - 1) & 1), abort, a.status))) break;
+                    if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&full[s], 2 * SLOT);
+                    if (kch < HD / 64)
+                        pair_load_4d(base + s * SLOT + kdst, &tmk, kch * 64, xk & (ps - 1), w.j, page, pair_bar(&full[s], 0));
+                    ++g;
+                }
+                if (i >= NB) {
+                    const int x0 = (w.first() + i - NB) * KT, s = g % NS, page = page_of((x0 >> shift) + vpg);
+                    if (g >= NS && !(ok = pa_warp_wait(&empty[s], (uint32_t)((g / NS - 1) & 1), abort, a.status))) break;
+                    if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&full[s], 2 * SLOT);
+                    if (vch < L::VC / 64)
+                        pair_load_4d(base + s * SLOT + vdst, &tmv, rank * L::VC + vch * 64, x0 & (ps - 1), w.j, page,
+                                     pair_bar(&full[s], 0));
+                    ++g;
+                }
+            }
+        }
+        // every copy lands before the pair's shared memory is released (bounded)
+        if (rank == 0) {
+            if (item > 0) mbar_wait_bounded(qfull, (uint32_t)((item - 1) & 1), a.status, 5);
+            for (int i = max(0, g - NS); i < g; ++i) mbar_wait_bounded(&full[i % NS], (uint32_t)((i / NS) & 1), a.status, 5);
+        }
+    } else if (warp == PA_ISSUER) {
+        fewer_registers();
+        if (lane == 0 && rank == 1) {
+            // the first CTA's last arrival here
+            mbar_wait_bounded(drain, 0u, a.status, 5);
+        } else if (lane == 0) {
+            // This thread's code is kept small: what it does between two products
+            // is time the tensor cores wait, and the softmax warps' code fills
+            // the instruction cache.
+            constexpr uint32_t id_s = umma_idesc_f16<BF, 256, KT, false>(), id_o = umma_idesc_f16<BF, 256, HD, true>();
+            const uint64_t kdesc = umma_desc128(smem_u32(ring), 16), vdesc = umma_desc128(smem_u32(ring), KT * 128),
+                           qdesc = umma_desc128(smem_u32(smem), 16);
+            int t = 0, slot = 0, item = 0;  // t: of the next scores
+            uint32_t phase = 0;             // of the slot
+            bool ok = true;
+            auto next_landed = [&] { return pa_wait(&full[slot], phase, abort, a.status); };
+            auto used = [&] {
+                pair_commit(&empty[slot]);
+                if (++slot == NS) slot = 0, phase ^= 1;
+            };
+            for (; ok && w.more(); w.next()) {
+                const int n = w.tiles();
+                if (n == 0) continue;
+                if (!(ok = pa_wait(qfull, (uint32_t)(item & 1), abort, a.status))) break;
+                // NB products of Q and K ahead of P V: the scores that the softmax warps will want next
+                for (int i = 0; i < n + NB; ++i) {
+                    if (i < n) {
+                        // S of tile t, once its buffer has been read and the keys are there
+                        if (t >= NB && !(ok = pa_wait(&sfree[(t - NB) & 1], (uint32_t)(((t - NB) >> 1) & 1), abort, a.status))) break;
+                        if (!(ok = next_landed())) break;
+                        tc_fence_after();
+                        uint64_t kd = kdesc + (uint64_t)(slot * (SLOT / 16)), qd = qdesc;
+                        const uint32_t d = tmem + L::S + (NB == 2 ? (t & 1) * KT : 0);
+#pragma unroll 1
+                        for (int ch = 0; ch < HD / 64; ++ch, kd += L::KR * 128 / 16, qd += PA_ROWS * 128 / 16)
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) umma_f16_ss2(d, qd + 2 * kk, kd + 2 * kk, id_s, ch > 0 || kk > 0);
+                        pair_commit(&sfull[t & 1]);
+                        used();
+                        if (i + 1 == n) pair_commit(qempty);
+                        ++t;
+                    }
+                    if (i < NB) continue;
+                    const int tv = t - 1 - (i < n ? NB : n + NB - 1 - i);
+                    if (!(ok = pa_wait(&pfull[tv & 1], (uint32_t)((tv >> 1) & 1), abort, a.status) && next_landed())) break;
+                    // O of the item before has been read
+                    if (i == NB && item > 0 && !(ok = pa_wait(oread, (uint32_t)((item - 1) & 1), abort, a.status))) break;
+                    tc_fence_after();
+                    uint64_t vd = vdesc + (uint64_t)(slot * (SLOT / 16));
+                    uint32_t pc = tmem + L::P + (tv & 1) * (KT / 2);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half, vd += 4 * 128, pc += 32)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16_ts<true>(tmem + L::O, pc + 8 * kk, vd + 128 * kk, id_o, i > NB || half > 0 || kk > 0);
+                    used();
+                    pair_commit(&pdone[tv & 1]);
+                }
+                ++item;
+            }
+            // every MMA issued above (bounded, even after an abort)
+            pair_commit(drain);
+            mbar_wait_bounded(drain, 0u, a.status, 5);
+        }
+        __syncwarp();
+    } else if (warp >= PA_SOFTMAX) {
+        fewer_registers();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_SOFTMAX));
+        // row = TMEM lane; warps 0-3 take the even tiles, warps 4-7 the odd ones
+        const int quarter = warp & 3, wg = warp >> 2, row = 32 * quarter + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
+        const float c = a.scale * 1.44269504088896340736f;  // log2 e
+        int t0 = 0, g0 = 0, u0 = 0, told = 0, zeroed = 0;  // u0: tiles of this quarter so far (of items where it has live rows)
+        bool ok = true;
+        PaItem tail = {0, 0, 0, 0};
+        // m after tile u of this quarter, from the warp that has the tile to the
+        // other: a word with its tile's number, so that no barrier is needed
+        auto publish = [&](int u, float m) {
+            const uint2 v = make_uint2(__float_as_uint(m), (uint32_t)u + 1);
+            asm volatile("st.volatile.shared.v2.u32 [%0], {%1, %2};" ::"r"(smem_u32(&sh.m[u & 1][row])), "r"(v.x), "r"(v.y) : "memory");
+        };
+        auto follow = [&](int u, float &m) { return pair_follow(&sh.m[u & 1][row], (uint32_t)u + 1, m, abort, a.status); };
+        // arrivals that both CTAs' warps make in the first
+        auto arrive = [&](uint64_t *bar) {
+            if (rank == 0) mbar_arrive(bar);
+            else pair_arrive(bar);
+        };
+        for (; ok && w.more(); w.next()) {
+            const int n = w.tiles(), i0 = w.r * tqw + rank * tq, i = i0 + row / G;
+            const int rows = max(0, min(tq, w.s.q_n - i0)) * G;
+            const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
+            // a dead row's scores are garbage that no one reads
+            const int hi = live ? w.s.base + i + 1 : 0x7fffffff;
+            const int lo = live && a.window > 0 ? max(0, hi - a.window) : 0;
+            float m = -INFINITY, l = 0.0f;  // m in units of c s; l of this warp's tiles
+            for (int k = (wg ^ t0) & 1; k < n; k += 2) {
+                const int t = t0 + k, x0 = (w.first() + k) * KT;
+                if (!(ok = pa_warp_wait(&sfull[wg], (uint32_t)((t >> 1) & 1), abort, a.status))) break;
+                if (idle) {
+                    if (lane == 0) arrive(&sfree[wg]);
+                } else {
+                    tc_fence_after();
+                    float s[KT];
+#pragma unroll
+                    for (int x = 0; x < KT / 32; ++x) tmem_ld32(lane_base + L::S + (NB == 2 ? wg * KT : 0) + 32 * x, (uint32_t *)s + 32 * x);
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(&sfree[wg]);
+                    if (__any_sync(0xffffffffu, x0 < lo || x0 + KT > hi)) {
+#pragma unroll
+                        for (int x = 0; x < KT; ++x)
+                            if (x0 + x < lo || x0 + x >= hi) s[x] = -INFINITY;
+                    }
+                    float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int x = 4; x < KT; x += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            tops[e] = x + 4 + e < KT ? max3(tops[e], s[x + e], s[x + 4 + e]) : fmaxf(tops[e], s[x + e]);
+                    const float top = c * fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+                    // the other warps' m after the tile before, and ours
+                    float before = -INFINITY;
+                    if (k > 0 && !(ok = follow(u0 + k - 1, before))) break;
+                    const float now = top > before + PA_SLACK ? top : before;
+                    publish(u0 + k, now);
+                    if (m != now) {
+                        l *= m == -INFINITY ? 0.0f : ex2(m - now);
+                        m = now;
+                    }
+                    if (k > 0 && __any_sync(0xffffffffu, now != before)) {
+                        // O, once the products so far are done
+                        if (!(ok = pa_warp_wait(&pdone[wg ^ 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status))) break;
+                        tc_fence_after();
+                        const float f = before == -INFINITY ? 1.0f : ex2(before - now);
+#pragma unroll 1
+                        for (int x = 0; x < HD / 32; ++x) {
+                            uint32_t v[32];
+                            tmem_ld32(lane_base + L::O + 32 * x, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tmem_st32(lane_base + L::O + 32 * x, v);
+                        }
+                        tmem_wait_st();
+                    }
+                    const float mm = m == -INFINITY ? 0.0f : m;
+                    const uint64_t c2 = pack2(c, c), m2 = pack2(-mm, -mm);
+                    uint64_t sum[2] = {0, 0};
+                    // P's buffer is free once the product of two tiles ago is done
+                    if (t >= 2 && !(ok = pa_warp_wait(&pdone[wg], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status))) break;
+#pragma unroll
+                    for (int x = 0; x < KT / 64; ++x) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float2 y = unpack2(fma2(pack2(s[64 * x + 2 * e], s[64 * x + 2 * e + 1]), c2, m2));
+                            const float p0 = ex2(y.x), p1 = ex2(y.y);
+                            sum[e & 1] = add2(sum[e & 1], pack2(p0, p1));
+                            p[e] = Half16<BF>::down(p0, p1);
+                        }
+                        tmem_st32(lane_base + L::P + wg * (KT / 2) + 32 * x, p);
+                    }
+                    const float2 both = unpack2(add2(sum[0], sum[1]));
+                    l += both.x + both.y;
+                }
+                // values of positions that no row of the item sees
+                if (x0 < w.sp.lo || x0 + KT > w.sp.hi) {
+                    const int g = g0 + min(n, k + 1 + NB) + k;  // V's slot: after K of NB tiles more
+                    // the first CTA sees the copies of both land, and tells the
+                    // second; not before tile t - 2 is done with in both, so
+                    // that what it tells is not overtaken
+                    if (t >= 2 && !(ok = pa_warp_wait(&pdone[wg], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status))) break;
+                    if (rank == 0) {
+                        if (!(ok = pa_warp_wait(&full[g % NS], (uint32_t)((g / NS) & 1), abort, a.status))) break;
+                        if (quarter == 0 && lane == 0) pair_arrive(&vlanded[wg], 1);
+                    } else if (!(ok = pa_warp_wait(&vlanded[wg], (uint32_t)(zeroed++ & 1), abort, a.status))) break;
+                    uint8_t *v = ring + (size_t)(g % NS) * SLOT;
+                    for (int e = tid & 127; e < SLOT / 16; e += 128) {
+                        const int x = (e >> 3) % KT;
+                        if (x0 + x < w.sp.lo || x0 + x >= w.sp.hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(&pfull[wg]);
+            }
+            if (!ok) break;
+            if (n > 0) {
+                const int last = t0 + n - 1;
+                if (!(ok = pa_warp_wait(&pdone[last & 1], (uint32_t)((last >> 1) & 1), abort, a.status))) break;
+                tc_fence_after();
+                if (!idle) {
+                    // m of the last tile, and the other warp's sum under it
+                    float end = m, theirs;
+                    if ((last & 1) != wg && !(ok = follow(u0 + n - 1, end))) break;
+                    l *= m == end ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - end);
+                    m = end;
+                    const int turn = told++ & 1;
+                    sh.half[turn][wg][row] = l;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pair[quarter]);
+                    if (!(ok = pa_warp_wait(&pair[quarter], (uint32_t)turn, abort, a.status))) break;
+                    theirs = *(volatile float *)&sh.half[turn][wg ^ 1][row];
+                    l = wg ? theirs + l : l + theirs;
+                    u0 += n;
+                }
+            }
+            pa_write<HD, BF>(a, w, sh.run, me, blockIdx.x, w.s.q_lo + i0, G, rows, row, wg, n > 0, m, l, lane_base + L::O, tail);
+            if (n > 0) {
+                __syncwarp();
+                if (lane == 0) arrive(oread);
+            }
+            t0 += n;
+            g0 += 2 * n;
+        }
+        if (tid == 0) a.items[blockIdx.x] = tail;
+    }
+    __syncwarp();
+    tc_fence_before();
+    pair_barrier();
+    if (warp == PA_ISSUER) {
+        __syncwarp();
+        tc_fence_after();
+        pair_tmem_free(tmem);
+    }
+}
+
+// Add up the records of item blockIdx.x (the tail of that CTA's run, if it has
+// one) and write its rows.  A group of SP threads takes eight values of a row;
+// thread p has parts p, p + SP, ..., four in flight, and the group adds its
+// sums up, all in an order that the sizes fix.
+template <int HD, bool BF, int SP>
+M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
+    const int G = a.n_q / a.kv.n_kv, p = threadIdx.x % SP;
+    const int first = blockIdx.x;
+    auto record = [&](int x) { return a.part + (size_t)(2 * (first + stride * x) + (x == 0 ? 1 : 0)) * pa_record(HD); };
+    const int n = it.rows * (HD / 8), per = 256 / SP;
+    for (int e0 = blockIdx.y * per; e0 < n; e0 += gridDim.y * per) {
+        const int e = min(n - 1, e0 + (int)threadIdx.x / SP), d8 = e / it.rows, row = e - d8 * it.rows;
+        float m = -INFINITY, l = 0.0f, o[8] = {};
+        for (int x0 = p; x0 < it.np; x0 += 4 * SP) {
+            float2 ml[4];
+            float4 y[4][2];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int x = x0 + q * SP;
+                const bool in = x < it.np;
+                const float *r = record(x);
+                ml[q] = in ? __ldcg((const float2 *)(r + (size_t)PA_ROWS * HD) + row) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+                    y[q][v] = in ? __ldcg((const float4 *)r + (size_t)(2 * d8 + v) * PA_ROWS + row) : make_float4(0, 0, 0, 0);
+            }
+            const float mn = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+            const float ref = mn == -INFINITY ? 0.0f : mn, f0 = ex2(m - ref);
+            m = mn;
+            l *= f0;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) o[v] *= f0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float f = ex2(ml[q].x - ref);
+                l = fmaf(f, ml[q].y, l);
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    o[4 * v] = fmaf(f, y[q][v].x, o[4 * v]), o[4 * v + 1] = fmaf(f, y[q][v].y, o[4 * v + 1]);
+                    o[4 * v + 2] = fmaf(f, y[q][v].z, o[4 * v + 2]), o[4 * v + 3] = fmaf(f, y[q][v].w, o[4 * v + 3]);
+                }
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int d = 1; d < SP; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float f = ex2(m - (mx == -INFINITY ? 0.0f : mx));
+        l *= f;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) o[v] *= f;
+#pragma unroll
+        for (int d = 1; d < SP; d <<= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+            for (int v = 0; v < 8; ++v) o[v] += __shfl_xor_sync(0xffffffffu, o[v], d);
+        }
+        if (p != 0 || e0 + (int)threadIdx.x / SP >= n) continue;
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint32_t y[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[v] = Half16<BF>::down(o[2 * v] * inv, o[2 * v + 1] * inv);
+        const long long tok = it.tok + row / G;
+        const int h = it.j * G + row % G;
+        *(uint4 *)((uint16_t *)a.out + tok * a.out_stride + (long long)h * HD + 8 * d8) = make_uint4(y[0], y[1], y[2], y[3]);
+        if (d8 == 0 && a.lse)
+            a.lse[tok * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (mx + log2f(l)) : -INFINITY;
+    }
+}
+
+template <int HD, bool BF>
+__global__ void __launch_bounds__(256) k_paged_join(const AttnArgs a, int stride) {
+    pdl_wait();
+    pdl_trigger();
+    const PaItem it = a.items[blockIdx.x];
+    if (it.np == 0) return;
+    if (it.np <= 2) pa_join<HD, BF, 2>(a, it, stride);
+    else pa_join<HD, BF, 8>(a, it, stride);
 }
 
 namespace {
@@ -807,53 +1329,85 @@ PFN_cuTensorMapEncodeTiled_v12000 pa_encoder() {
 }
 
 // (value, slot, kv head, page) of a pool; a box is 64 values of `rows` slots.
-bool pa_map(CUtensorMap *tm, const M27BPagedKV &kv, const void *pool, int rows) {
+bool pa_pool_map(CUtensorMap *tm, const M27BPagedKV &kv, const void *pool, int rows) {
     auto enc = pa_encoder();
     if (!enc) return false;
     const cuuint64_t dim[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_pages};
     const cuuint64_t stride[3] = {(cuuint64_t)kv.n_kv * kv.head_dim * 2, (cuuint64_t)kv.head_dim * 2,
                                   (cuuint64_t)kv.page_stride * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(kv.page_size < rows ? kv.page_size : rows), 1, 1}, one[4] = {1, 1, 1, 1};
     return enc(tm, kv.type == M27B_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                const_cast<void *>(pool), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// (value, head, token) of q; a box is 64 values of the G heads of a kv head, tq tokens.
+bool pa_q_map(CUtensorMap *tm, const AttnArgs &a, int G, int tq) {
+    auto enc = pa_encoder();
+    if (!enc) return false;
+    const cuuint64_t dim[3] = {(cuuint64_t)a.kv.head_dim, (cuuint64_t)a.n_q, (cuuint64_t)a.bt.n_tok};
+    const cuuint64_t stride[2] = {(cuuint64_t)a.kv.head_dim * 2, (cuuint64_t)a.q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)tq}, one[3] = {1, 1, 1};
+    return enc(tm, a.kv.type == M27B_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+               const_cast<void *>(a.q), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
-// CTAs of a launch: one per SM of the current device.
+constexpr int PA_MAX_CTAS = 160;  // CTAs the scratch has records for
+
+// CTAs of a launch: one per SM of the current device, an even number.
 int pa_ctas() {
     static int sms[64] = {};
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return 0;
     if (dev < 64 && sms[dev]) return sms[dev];
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (n > PA_MAX_CTAS) n = PA_MAX_CTAS;
+    n = (n < PA_MAX_CTAS ? n : PA_MAX_CTAS) & ~1;
     if (dev < 64) sms[dev] = n;
     return n;
 }
-constexpr int PA_SCRATCH_CTAS = 160;  // most CTAs the scratch has records for
 
-template <int HD, bool BF>
-cudaError_t pa_launch(const AttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int ctas, cudaStream_t st) {
-    auto kern = k_paged_attn<HD, BF>;
-    static bool ready[64] = {};
+// Raise a kernel's shared-memory limit, once per device.
+template <class K>
+cudaError_t pa_ready(K kern, size_t smem, bool (&done)[64]) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64 || !ready[dev]) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaPlan<HD>::SMEM);
-        if (e != cudaSuccess) return e;
-        if (dev >= 0 && dev < 64) ready[dev] = true;
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+}
+
+template <int HD, bool BF>
+cudaError_t pa_launch(const AttnArgs &a, int G, bool pair, int ctas, cudaStream_t st, bool *maps) {
+    CUtensorMap tk, tv, tq;
+    cudaError_t e;
+    if constexpr (HD >= 128) {
+        if (pair) {
+            using L = PairPlan<HD>;
+            static bool ready[64] = {};
+            *maps = pa_pool_map(&tk, a.kv, a.kv.k, L::KR) && pa_pool_map(&tv, a.kv, a.kv.v, L::KT) && pa_q_map(&tq, a, G, PA_ROWS / G);
+            if (!*maps) return cudaSuccess;
+            e = pa_ready(k_paged_attn_pair<HD, BF>, L::SMEM, ready);
+            if (e == cudaSuccess) e = launch_pdl(k_paged_attn_pair<HD, BF>, dim3(ctas), dim3(PAIR_THREADS), L::SMEM, st, a, tk, tv, tq);
+            return e != cudaSuccess ? e : launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 8), dim3(256), 0, st, a, 2);
+        }
     }
-    return launch_pdl(kern, dim3(ctas), dim3(PA_THREADS), PaPlan<HD>::SMEM, st, a, k, v);
+    using L = PaPlan<HD>;
+    static bool ready[64] = {};
+    *maps = pa_pool_map(&tk, a.kv, a.kv.k, L::KT) && pa_pool_map(&tv, a.kv, a.kv.v, L::KT);
+    if (!*maps) return cudaSuccess;
+    e = pa_ready(k_paged_attn<HD, BF>, L::SMEM, ready);
+    if (e == cudaSuccess) e = launch_pdl(k_paged_attn<HD, BF>, dim3(ctas), dim3(PA_THREADS), L::SMEM, st, a, tk, tv);
+    return e != cudaSuccess ? e : launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 8), dim3(256), 0, st, a, 1);
 }
 
 template <bool BF>
-cudaError_t pa_launch_hd(const AttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int ctas, cudaStream_t st) {
+cudaError_t pa_launch_hd(const AttnArgs &a, int G, bool pair, int ctas, cudaStream_t st, bool *maps) {
     switch (a.kv.head_dim) {
-    case 64: return pa_launch<64, BF>(a, k, v, ctas, st);
-    case 128: return pa_launch<128, BF>(a, k, v, ctas, st);
-    default: return pa_launch<256, BF>(a, k, v, ctas, st);
+    case 64: return pa_launch<64, BF>(a, G, pair, ctas, st, maps);
+    case 128: return pa_launch<128, BF>(a, G, pair, ctas, st, maps);
+    default: return pa_launch<256, BF>(a, G, pair, ctas, st, maps);
     }
 }
 
@@ -867,7 +1421,7 @@ extern "C" {
 size_t m27b_paged_attn_scratch_bytes(int n_q, int n_kv, int head_dim) {
     if (n_kv < 1 || n_kv > 1024 || n_q < n_kv || n_q % n_kv || n_q / n_kv > 128) return 0;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-    return PA_MAX_CTAS * sizeof(unsigned) + 2 * PA_SCRATCH_CTAS * pa_record(head_dim) * sizeof(float);
+    return PA_MAX_CTAS * sizeof(PaItem) + 2 * PA_MAX_CTAS * pa_record(head_dim) * sizeof(float);
 }
 
 bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const void *q, long long q_stride, int n_q,
@@ -886,19 +1440,17 @@ bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const v
         return paged_fail(err, err_cap, "%s: token strides must be multiples of 8, at least n_q x head_dim", what);
     if (!(scale > 0.0f) || scale > 1e30f) return paged_fail(err, err_cap, "%s: scale must be positive and finite", what);
     if (kv->page_stride >= 1ll << 39) return paged_fail(err, err_cap, "%s: page_stride (%lld) too large", what, kv->page_stride);
-    const int rows = kv->head_dim == 256 ? (kv->page_size < 64 ? kv->page_size : 64) : (kv->page_size < 128 ? kv->page_size : 128);
-    CUtensorMap tk, tv;
-    if (!pa_map(&tk, *kv, kv->k, rows) || !pa_map(&tv, *kv, kv->v, rows))
-        return paged_fail(err, err_cap, "%s: the pools' tensor maps were refused", what);
-    int ctas = pa_ctas();
-    if (ctas < 1) return paged_fail(err, err_cap, "%s: no CUDA device", what);
-    if (ctas > PA_SCRATCH_CTAS) ctas = PA_SCRATCH_CTAS;
+    const int ctas = pa_ctas(), G = n_q / kv->n_kv;
+    if (ctas < 2) return paged_fail(err, err_cap, "%s: no CUDA device", what);
     const AttnArgs a = {*kv, *batch, q, out, lse, q_stride, out_stride, n_q, window > 0 ? window : 0, scale,
-                        (unsigned *)scratch, (float *)((char *)scratch + PA_MAX_CTAS * sizeof(unsigned)),
-                        status_ptr_current()};
-    return paged_ok(kv->type == M27B_TYPE_BF16 ? pa_launch_hd<true>(a, tk, tv, ctas, stream)
-                                               : pa_launch_hd<false>(a, tk, tv, ctas, stream),
-                    what, err, err_cap);
+                        (PaItem *)scratch, (float *)((char *)scratch + PA_MAX_CTAS * sizeof(PaItem)), status_ptr_current()};
+    // pairs of CTAs when a sequence has rows for both, on average
+    const bool pair = (long long)batch->n_tok * G >= 256ll * batch->n_seq;
+    bool maps = false;
+    const cudaError_t e = kv->type == M27B_TYPE_BF16 ? pa_launch_hd<true>(a, G, pair, ctas, stream, &maps)
+                                                     : pa_launch_hd<false>(a, G, pair, ctas, stream, &maps);
+    if (e == cudaSuccess && !maps) return paged_fail(err, err_cap, "%s: the tensor maps were refused", what);
+    return paged_ok(e, what, err, err_cap);
 }
 
 }  // extern "C"

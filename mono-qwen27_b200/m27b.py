@@ -980,12 +980,12 @@ def rope_append(kv, q, k, v, cu_q, lens, rope, q_out, interleaved=False, q_norm=
 
 
 def paged_attn_scratch(n_q, n_kv, head_dim, device="cuda"):
-    """Scratch of paged_attn (zeroed; one for each stream that calls it)."""
+    """Scratch of paged_attn (one for each stream that calls it)."""
     import torch
     n = _paged_lib().m27b_paged_attn_scratch_bytes(n_q, n_kv, head_dim)
     if n == 0:
         raise M27BError(f"paged_attn: unsupported heads ({n_q} on {n_kv}, head_dim {head_dim})")
-    return torch.zeros(n, dtype=torch.uint8, device=device)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def paged_attn(kv, q, cu_q, lens, out, scratch, scale=None, window=0, lse=None, rows=None, stream=None):

@@ -87,7 +87,8 @@ def _check_attn(torch, m27b, q_lens, kv_lens, n_q, n_kv, hd, dtype, ps, window=0
     out = out_w[:, :n_q]
     ls = torch.full((total, n_q), 7.0, device="cuda") if lse else None
     scr = m27b.paged_attn_scratch(n_q, n_kv, hd)
-    for _ in range(2):  # the second call finds the scratch as the first left it
+    scr.fill_(255)
+    for _ in range(2):  # the scratch may hold anything
         m27b.paged_attn(c.kv, q, _cu(torch, q_lens), c.lens, out, scr, scale=scale, window=window, lse=ls, rows=c.rows_t)
     torch.cuda.synchronize()
     sc, u = hd ** -0.5 if scale is None else scale, P.U[dtype]
@@ -107,7 +108,6 @@ def _check_attn(torch, m27b, q_lens, kv_lens, n_q, n_kv, hd, dtype, ps, window=0
         at += n
     if strided:
         assert (_np(out_w)[:, n_q:] == 7.0).all()
-    assert int(scr.view(torch.uint8)[:4096].sum()) == 0
     assert m27b.device_status() == 0
 
 
