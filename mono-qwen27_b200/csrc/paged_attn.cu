@@ -101,33 +101,40 @@ __host__ __device__ constexpr size_t pa_record(int hd) { return (size_t)PA_ROWS 
 
 // ---- tensor core helpers ----
 
-// D[tmem] (+)= A[tmem] B[smem], 16-bit operands, fp32 sums, one thread; for a pair, both CTAs' halves.
-template <bool PAIR>
+// D[tmem] (+)= A[tmem] B[smem], 16-bit operands, fp32 sums, one thread.
 M27B_DI void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    if constexpr (PAIR)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                     "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                     : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                     "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                     : "memory");
-}
-// The same with A in shared memory, for a pair.
-M27B_DI void umma_f16_ss2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
                  : "memory");
 }
-// The MMAs that this thread issued for the pair arrive on `bar` of both CTAs when they complete.
-M27B_DI void pair_commit(uint64_t *bar) {
+// For a pair: D of both CTAs, A in TMEM or shared memory of each, B half in
+// each.  The whole warp comes here and the lane with `lead` issues: operands
+// that are the same in all lanes stay in uniform registers, which the
+// instruction reads.
+M27B_DI void pair_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+                 : "memory");
+}
+M27B_DI void pair_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+                 : "memory");
+}
+M27B_DI uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+// The MMAs that the lead lane issued for the pair arrive on `bar` of both CTAs when they complete.
+M27B_DI void pair_commit(uint32_t lead, uint32_t bar) {
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_u32(bar)),
-        "h"((uint16_t)3)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+        "h"((uint16_t)3), "r"(lead)
         : "memory");
 }
 M27B_DI void pair_tmem_alloc(uint32_t *slot) {
@@ -473,8 +480,43 @@ M27B_DI bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *s
         if ((it & 63u) == 0 && pa_give_up(t0, abort, status)) return false;
     return true;
 }
+// The same for a barrier's shared-memory address.
+M27B_DI bool pa_wait_at(uint32_t bar, uint32_t parity, volatile int *abort, int *status) {
+    unsigned long long t0 = 0;
+    for (unsigned it = 1;; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((it & 63u) == 0 && pa_give_up(t0, abort, status)) return false;
+    }
+}
 M27B_DI bool pa_warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
     return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, status)) != 0;
+}
+
+// Lanes 4 g + i hold y[j] = element (i, j) of a 4 x 4 matrix of 16-byte
+// elements; afterwards element (j, i).
+M27B_DI void transpose4(uint4 (&y)[4]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int b = 1; b < 4; b <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (!(j & b)) {
+                // swap y[j | b] of lanes without bit b and y[j] of lanes with it
+                const bool up = lane & b;
+                uint4 give = up ? y[j] : y[j | b], got;
+                got.x = __shfl_xor_sync(0xffffffffu, give.x, b), got.y = __shfl_xor_sync(0xffffffffu, give.y, b);
+                got.z = __shfl_xor_sync(0xffffffffu, give.z, b), got.w = __shfl_xor_sync(0xffffffffu, give.w, b);
+                if (up) y[j] = got;
+                else y[j | b] = got;
+            }
 }
 
 // The end of an item in this worker's run: this thread's half of its row's O
@@ -490,7 +532,6 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
     if (w.whole()) {
         if (idle) return;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        uint16_t *op = (uint16_t *)a.out + at * a.out_stride + (long long)h * HD + half * (HD / 2);
 #pragma unroll 1
         for (int x = 0; x < HD / 64; ++x) {
             uint32_t v[32];
@@ -498,17 +539,27 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
                 tmem_ld32(o + half * (HD / 2) + 32 * x, v);
                 tmem_wait_ld();
             }
-            if (live)
+            // four quadruples of 16 bits; then lane 4 g + j holds quadruple j of rows
+            // 4 g .. 4 g + 3, so that a store has 64 bytes of a row together
+            uint4 y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t y[4];
+            for (int e = 0; e < 4; ++e) {
+                uint32_t z[4];
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        y[d] = l > 0.0f ? Half16<BF>::down(__uint_as_float(v[8 * e + 2 * d]) * inv,
-                                                           __uint_as_float(v[8 * e + 2 * d + 1]) * inv)
-                                        : 0u;
-                    *((uint4 *)(op + 32 * x) + e) = make_uint4(y[0], y[1], y[2], y[3]);
-                }
+                for (int d = 0; d < 4; ++d)
+                    z[d] = l > 0.0f ? Half16<BF>::down(__uint_as_float(v[8 * e + 2 * d]) * inv,
+                                                       __uint_as_float(v[8 * e + 2 * d + 1]) * inv)
+                                    : 0u;
+                y[e] = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+            transpose4(y);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int other = (row & ~3) + r;
+                if (other < rows)
+                    *(uint4 *)((uint16_t *)a.out + (tok + other / G) * a.out_stride + (long long)(w.j * G + other % G) * HD +
+                               half * (HD / 2) + 32 * x + 8 * (row & 3)) = y[r];
+            }
         }
         if (live && a.lse && half == 0)
             a.lse[at * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
@@ -640,7 +691,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     const uint32_t k = base + (g % NS) * SLOT;
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk)
-                        umma_f16_ts<false>(tmem + L::S, tmem + L::Q + kk * 8,
+                        umma_f16_ts(tmem + L::S, tmem + L::Q + kk * 8,
                                            umma_desc128(k + (kk / 4) * (KT * 128) + (kk % 4) * 32, 16), id_s, kk > 0);
                     umma_commit(sfull);
                     umma_commit(&empty[g % NS]);
@@ -657,7 +708,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     const uint32_t v = base + (g % NS) * SLOT;
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
-                        umma_f16_ts<false>(tmem + L::O, tmem + L::P + (t & 1) * (KT / 2) + kk * 8,
+                        umma_f16_ts(tmem + L::O, tmem + L::P + (t & 1) * (KT / 2) + kk * 8,
                                            umma_desc128(v + kk * 2048, KT * 128), id_o, i > 0 || kk > 0);
                     umma_commit(&empty[g % NS]);
                     umma_commit(&pdone[t & 1]);
@@ -963,12 +1014,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         for (; ok && w.more(); w.next()) {
             const int n = w.tiles();
             if (n == 0) continue;
-            if (item > 0 && !(ok = pa_warp_wait(qempty, (uint32_t)((item - 1) & 1), abort, a.status))) break;
-            if (lane == 0 && rank == 0) mbar_arrive_expect_tx(qfull, 2 * (HD / 64) * G * tq * 128);
-            if (lane < HD / 64)
-                pair_load_3d(smem_u32(smem) + lane * (PA_ROWS * 128), &tmq, lane * 64, w.j * G,
-                             w.s.q_lo + w.r * tqw + rank * tq, pair_bar(qfull, 0));
-            ++item;
             const int *ids = a.kv.table + (long long)w.s.row * a.kv.n_cols;
             int have = -32, cur = 0;  // lane's page id of page have + lane of the sequence
             auto page_of = [&](int p) { return __shfl_sync(0xffffffffu, cur, (p - have) & 31); };
@@ -986,6 +1031,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     if (kch < HD / 64)
                         pair_load_4d(base + s * SLOT + kdst, &tmk, kch * 64, xk & (ps - 1), w.j, page, pair_bar(&full[s], 0));
                     ++g;
+                }
+                if (i == 0) {
+                    // Q, once the last product with the item's before is done
+                    if (item > 0 && !(ok = pa_warp_wait(qempty, (uint32_t)((item - 1) & 1), abort, a.status))) break;
+                    if (lane == 0 && rank == 0) mbar_arrive_expect_tx(qfull, 2 * (HD / 64) * G * tq * 128);
+                    if (lane < HD / 64)
+                        pair_load_3d(smem_u32(smem) + lane * (PA_ROWS * 128), &tmq, lane * 64, w.j * G,
+                                     w.s.q_lo + w.r * tqw + rank * tq, pair_bar(qfull, 0));
+                    ++item;
                 }
                 if (i >= NB) {
                     const int x0 = (w.first() + i - NB) * KT, s = g % NS, page = page_of((x0 >> shift) + vpg);
@@ -1005,68 +1059,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         }
     } else if (warp == PA_ISSUER) {
         fewer_registers();
-        if (lane == 0 && rank == 1) {
-            // the first CTA's last arrival here
-            mbar_wait_bounded(drain, 0u, a.status, 5);
-        } else if (lane == 0) {
-            // This thread's code is kept small: what it does between two products
-            // is time the tensor cores wait, and the softmax warps' code fills
-            // the instruction cache.
+        if (rank == 0) {
+            // The warp stays together and one lane issues; its code is kept
+            // small: what it does between two products is time the tensor
+            // cores wait.
             constexpr uint32_t id_s = umma_idesc_f16<BF, 256, KT, false>(), id_o = umma_idesc_f16<BF, 256, HD, true>();
+            const uint32_t lead = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint64_t kdesc = umma_desc128(smem_u32(ring), 16), vdesc = umma_desc128(smem_u32(ring), KT * 128),
                            qdesc = umma_desc128(smem_u32(smem), 16);
-            int t = 0, slot = 0, item = 0;  // t: of the next scores
-            uint32_t phase = 0;             // of the slot
+            const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), sfull0 = smem_u32(sfull), sfree0 = smem_u32(sfree),
+                           pfull0 = smem_u32(pfull), pdone0 = smem_u32(pdone);
+            uint32_t t = 0, slot = 0, phase = 0, item = 0;  // t: tile of the next scores; phase: of the slot
             bool ok = true;
-            auto next_landed = [&] { return pa_wait(&full[slot], phase, abort, a.status); };
             auto used = [&] {
-                pair_commit(&empty[slot]);
+                pair_commit(lead, empty0 + 8 * slot);
                 if (++slot == NS) slot = 0, phase ^= 1;
             };
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                return ok = __all_sync(0xffffffffu, pa_wait_at(bar, parity, abort, a.status)) != 0;
+            };
             for (; ok && w.more(); w.next()) {
-                const int n = w.tiles();
+                const int n = __shfl_sync(0xffffffffu, w.tiles(), 0);
                 if (n == 0) continue;
-                if (!(ok = pa_wait(qfull, (uint32_t)(item & 1), abort, a.status))) break;
+                if (!wait(smem_u32(qfull), item & 1)) break;
                 // NB products of Q and K ahead of P V: the scores that the softmax warps will want next
                 for (int i = 0; i < n + NB; ++i) {
                     if (i < n) {
                         // S of tile t, once its buffer has been read and the keys are there
-                        if (t >= NB && !(ok = pa_wait(&sfree[(t - NB) & 1], (uint32_t)(((t - NB) >> 1) & 1), abort, a.status))) break;
-                        if (!(ok = next_landed())) break;
+                        const uint32_t u = t - NB;
+                        if (t >= NB && !wait(sfree0 + 8 * (u & 1), (u >> 1) & 1)) break;
+                        if (!wait(full0 + 8 * slot, phase)) break;
                         tc_fence_after();
                         uint64_t kd = kdesc + (uint64_t)(slot * (SLOT / 16)), qd = qdesc;
-                        const uint32_t d = tmem + L::S + (NB == 2 ? (t & 1) * KT : 0);
+                        const uint32_t d = tm + L::S + (NB == 2 ? (t & 1) * KT : 0);
 #pragma unroll 1
                         for (int ch = 0; ch < HD / 64; ++ch, kd += L::KR * 128 / 16, qd += PA_ROWS * 128 / 16)
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk) umma_f16_ss2(d, qd + 2 * kk, kd + 2 * kk, id_s, ch > 0 || kk > 0);
-                        pair_commit(&sfull[t & 1]);
+                            for (int kk = 0; kk < 4; ++kk) pair_mma_ss(lead, d, qd + 2 * kk, kd + 2 * kk, id_s, ch > 0 || kk > 0);
+                        pair_commit(lead, sfull0 + 8 * (t & 1));
                         used();
-                        if (i + 1 == n) pair_commit(qempty);
+                        if (i + 1 == n) pair_commit(lead, smem_u32(qempty));
                         ++t;
                     }
                     if (i < NB) continue;
-                    const int tv = t - 1 - (i < n ? NB : n + NB - 1 - i);
-                    if (!(ok = pa_wait(&pfull[tv & 1], (uint32_t)((tv >> 1) & 1), abort, a.status) && next_landed())) break;
+                    const uint32_t v = t - 1 - (i < n ? NB : n + NB - 1 - i);
+                    if (!wait(pfull0 + 8 * (v & 1), (v >> 1) & 1)) break;
+                    if (!wait(full0 + 8 * slot, phase)) break;
                     // O of the item before has been read
-                    if (i == NB && item > 0 && !(ok = pa_wait(oread, (uint32_t)((item - 1) & 1), abort, a.status))) break;
+                    if (i == NB && item > 0 && !wait(smem_u32(oread), (item - 1) & 1)) break;
                     tc_fence_after();
                     uint64_t vd = vdesc + (uint64_t)(slot * (SLOT / 16));
-                    uint32_t pc = tmem + L::P + (tv & 1) * (KT / 2);
+                    uint32_t pc = tm + L::P + (v & 1) * (KT / 2);
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half, vd += 4 * 128, pc += 32)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16_ts<true>(tmem + L::O, pc + 8 * kk, vd + 128 * kk, id_o, i > NB || half > 0 || kk > 0);
+                            pair_mma_ts(lead, tm + L::O, pc + 8 * kk, vd + 128 * kk, id_o, i > NB || half > 0 || kk > 0);
                     used();
-                    pair_commit(&pdone[tv & 1]);
+                    pair_commit(lead, pdone0 + 8 * (v & 1));
                 }
                 ++item;
             }
             // every MMA issued above (bounded, even after an abort)
-            pair_commit(drain);
-            mbar_wait_bounded(drain, 0u, a.status, 5);
+            pair_commit(lead, smem_u32(drain));
         }
+        // (the second CTA: the first one's last arrival here)
+        mbar_wait_bounded(drain, 0u, a.status, 5);
         __syncwarp();
     } else if (warp >= PA_SOFTMAX) {
         fewer_registers();
@@ -1187,7 +1245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                         if (x0 + x < w.sp.lo || x0 + x >= w.sp.hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async();
-                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                    if (rank == 1) asm volatile("fence.acq_rel.cluster;" ::: "memory");
                 }
                 tmem_wait_st();
                 tc_fence_before();
