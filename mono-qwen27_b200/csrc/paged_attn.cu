@@ -200,6 +200,15 @@ M27B_DI void tmem_ld32(uint32_t taddr, uint32_t *v) {
         : "r"(taddr)
         : "memory");
 }
+M27B_DI void tmem_ld16(uint32_t taddr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
 M27B_DI void tmem_st32(uint32_t taddr, const uint32_t *v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -308,25 +317,22 @@ M27B_DI long long div_count(long long x, long long y) {
     return (x | y) >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
 }
 
-// The item at hand and its neighbours, walked alike by every role.
+// The item at hand, walked alike by every role.
 template <int KT>
 struct PaWalk {
-    const AttnArgs &a;
-    int tq;
     long long u, end;
-    int b, j, r, off;
+    int tq, b, j, r, off;
+    int take;  // units of this item in this run
     PaSeq s;
     PaSpan sp;
-    int take;  // units of this item in this run
 
-    M27B_DI PaWalk(const AttnArgs &a_, const PaRun &run, int tq_) : a(a_), tq(tq_) {
-        u = run.begin, end = run.end, b = run.b, j = run.j, r = run.r, off = run.off;
+    M27B_DI void begin(const AttnArgs &a, const PaRun &run, int tq_) {
+        tq = tq_, u = run.begin, end = run.end, b = run.b, j = run.j, r = run.r, off = run.off;
         s = run.seq;
-        if (more()) span();
+        if (more()) span(a);
     }
     M27B_DI bool more() const { return u < end; }
-    M27B_DI void seq() { s = pa_seq(a, b, tq, false); }
-    M27B_DI void span() {
+    M27B_DI void span(const AttnArgs &a) {
         sp = pa_span<KT>(s, r, tq, a.window);
         take = (int)min((long long)(sp.units() - off), end - u);
     }
@@ -334,7 +340,7 @@ struct PaWalk {
     M27B_DI int tiles() const { return sp.kt1 > sp.kt0 ? take : 0; }
     M27B_DI int first() const { return sp.kt0 + off; }
     M27B_DI bool whole() const { return off == 0 && take == sp.units(); }
-    M27B_DI void next() {
+    M27B_DI void next(const AttnArgs &a) {
         u += take;
         off = 0;
         if (!more()) return;
@@ -343,12 +349,11 @@ struct PaWalk {
             if (++j == a.kv.n_kv) {
                 j = 0;
                 do {
-                    ++b;
-                    seq();
+                    s = pa_seq(a, ++b, tq, false);
                 } while (s.nrt == 0);  // units are left, so a sequence with tokens follows
             }
         }
-        span();
+        span(a);
     }
 };
 
@@ -462,27 +467,21 @@ M27B_DI int pa_page(const AttnArgs &a, const Walk &w, const int *ids, int p, int
     return a.kv.n_pages;
 }
 
-// Bounded waits.  The timer and the abort flag are looked at only after many
-// tests (a test may itself wait a while in hardware), out of line: what stands
-// between the roles' hand-offs is a test and a branch.
-__device__ __noinline__ bool pa_give_up(unsigned long long &t0, volatile int *abort, int *status) {
+// Bounded waits.  The timer (in 2^20 ns, one register) and the abort flag are
+// looked at only after many tests (a test may itself wait a while in
+// hardware): what stands between the roles' hand-offs is a test and a branch.
+// No function call: the softmax warps hold their scores in registers here.
+M27B_DI bool pa_give_up(uint32_t &t0, volatile int *abort, int *status) {
     if (*abort) return true;
-    const unsigned long long now = global_ns();
+    const uint32_t now = (uint32_t)(global_ns() >> 20) | 1u;
     if (t0 == 0) t0 = now;
-    if (now - t0 <= M27B_WAIT_NS) return false;
+    if (now - t0 <= (uint32_t)(M27B_WAIT_NS >> 20)) return false;
     *abort = 1;
     if (status) atomicCAS(status, 0, 5);
     return true;
 }
-M27B_DI bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
-    unsigned long long t0 = 0;
-    for (unsigned it = 1; !mbar_try_wait(bar, parity); ++it)
-        if ((it & 63u) == 0 && pa_give_up(t0, abort, status)) return false;
-    return true;
-}
-// The same for a barrier's shared-memory address.
 M27B_DI bool pa_wait_at(uint32_t bar, uint32_t parity, volatile int *abort, int *status) {
-    unsigned long long t0 = 0;
+    uint32_t t0 = 0;
     for (unsigned it = 1;; ++it) {
         uint32_t ok;
         asm volatile(
@@ -495,6 +494,9 @@ M27B_DI bool pa_wait_at(uint32_t bar, uint32_t parity, volatile int *abort, int 
         if (ok) return true;
         if ((it & 63u) == 0 && pa_give_up(t0, abort, status)) return false;
     }
+}
+M27B_DI bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    return pa_wait_at(smem_u32(bar), parity, abort, status);
 }
 M27B_DI bool pa_warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
     return __all_sync(0xffffffffu, pa_wait(bar, parity, abort, status)) != 0;
@@ -519,13 +521,14 @@ M27B_DI void transpose4(uint4 (&y)[4]) {
             }
 }
 
-// The end of an item in this worker's run: this thread's half of its row's O
-// (columns [half HD / 2, ..) of TMEM at `o`) to the output, or, if the worker
+// The end of an item in this worker's run: this thread's part of its row's O
+// (columns [part HD / PARTS, ..) of TMEM at `o`) to the output, or, if the worker
 // has a part of the item only, O, m and l to its record.  `tok`: the first
 // token row of the CTA's rows; `any`: there were tiles (else O is 0).
-template <int HD, bool BF, class Walk>
+template <int HD, bool BF, int PARTS, class Walk>
 M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me, int cta, int tok, int G, int rows, int row,
-                      int half, bool any, float m, float l, uint32_t o, PaItem &tail) {
+                      int part, bool any, float m, float l, uint32_t o, PaItem &tail) {
+    constexpr int COLS = HD / PARTS;
     const bool live = row < rows, idle = (row & ~31) >= rows;
     const int h = w.j * G + row % G;
     const long long at = tok + row / G;
@@ -533,10 +536,10 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
         if (idle) return;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll 1
-        for (int x = 0; x < HD / 64; ++x) {
+        for (int x = 0; x < COLS / 32; ++x) {
             uint32_t v[32];
             if (any) {
-                tmem_ld32(o + half * (HD / 2) + 32 * x, v);
+                tmem_ld32(o + part * COLS + 32 * x, v);
                 tmem_wait_ld();
             }
             // four quadruples of 16 bits; then lane 4 g + j holds quadruple j of rows
@@ -558,10 +561,10 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
                 const int other = (row & ~3) + r;
                 if (other < rows)
                     *(uint4 *)((uint16_t *)a.out + (tok + other / G) * a.out_stride + (long long)(w.j * G + other % G) * HD +
-                               half * (HD / 2) + 32 * x + 8 * (row & 3)) = y[r];
+                               part * COLS + 32 * x + 8 * (row & 3)) = y[r];
             }
         }
-        if (live && a.lse && half == 0)
+        if (live && a.lse && part == 0)
             a.lse[at * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
     } else {
         // the item begins with worker c0 and ends with c1
@@ -572,17 +575,17 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
         if (idle) return;
         float *rec = a.part + (size_t)(2 * cta + (me == c0 ? 1 : 0)) * pa_record(HD);
 #pragma unroll 1
-        for (int x = 0; x < HD / 64; ++x) {
+        for (int x = 0; x < COLS / 32; ++x) {
             uint32_t v[32];
-            tmem_ld32(o + half * (HD / 2) + 32 * x, v);
+            tmem_ld32(o + part * COLS + 32 * x, v);
             tmem_wait_ld();
             if (live)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    __stcg((uint4 *)rec + (size_t)(half * (HD / 8) + 8 * x + e) * PA_ROWS + row,
+                    __stcg((uint4 *)rec + (size_t)(part * (COLS / 4) + 8 * x + e) * PA_ROWS + row,
                            make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
         }
-        if (live && half == 0) __stcg((float2 *)(rec + (size_t)PA_ROWS * HD) + row, make_float2(m, l));
+        if (live && part == 0) __stcg((float2 *)(rec + (size_t)PA_ROWS * HD) + row, make_float2(m, l));
     }
     tc_fence_before();
 }
@@ -630,7 +633,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    PaWalk<KT> w(a, sh.run, tq);
+    PaWalk<KT> w;
+    w.begin(a, sh.run, tq);
 
     if (warp == PA_PRODUCER) {
         const int ps = a.kv.page_size, shift = 31 - __clz(ps);
@@ -640,7 +644,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const uint32_t dst = ch * (KT * 128) + pg * rows * 128;
         int g = 0;
         bool ok = true;
-        for (; ok && w.more(); w.next()) {
+        for (; ok && w.more(); w.next(a)) {
             const int n = w.tiles();
             if (n == 0) continue;
             const int *ids = a.kv.table + (long long)w.s.row * a.kv.n_cols;
@@ -680,7 +684,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             int t0 = 0, g = 0, item = 0;
             bool ok = true;
             auto landed = [&](int g) { return pa_wait(&full[g % NS], (uint32_t)((g / NS) & 1), abort, a.status); };
-            for (; ok && w.more(); w.next()) {
+            for (; ok && w.more(); w.next(a)) {
                 const int n = w.tiles();
                 if (n == 0) continue;
                 // S of tile t = Q K^T, once S has been read and the keys are there
@@ -743,7 +747,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             theirs = *(volatile float *)&sh.half[turn][half ^ 1][row];
             return here;
         };
-        for (; ok && w.more(); w.next()) {
+        for (; ok && w.more(); w.next(a)) {
             const int n = w.tiles(), i0 = w.r * tq, i = i0 + row / G, h = w.j * G + row % G;
             const int rows = min(tq, w.s.q_n - i0) * G;
             const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
@@ -860,7 +864,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 if (!(ok = other(l, theirs))) break;
                 l = half ? theirs + l : l + theirs;
             }
-            pa_write<HD, BF>(a, w, sh.run, me, blockIdx.x, w.s.q_lo + i0, G, rows, row, half, n > 0, m, l, lane_base + L::O, tail);
+            pa_write<HD, BF, 2>(a, w, sh.run, me, blockIdx.x, w.s.q_lo + i0, G, rows, row, half, n > 0, m, l, lane_base + L::O, tail);
         }
         if (tid == 0) a.items[blockIdx.x] = tail;
     }
@@ -888,14 +892,22 @@ template <int HD> struct PairPlan {
     static_assert(P + KT <= 512, "TMEM plan");
     static_assert(SMEM > MMA_SMEM_MIN && SMEM <= MMA_SMEM_LIMIT - 8192, "one CTA per SM");
 };
-// Registers: the softmax warps hold a row of a tile; 2 x 128 threads of 216 and
-// 128 of 72 are the 384 x 168 that the block is launched with.
-constexpr int PAIR_THREADS = (PA_SOFTMAX + 4) * 32;
+// Warps 0-7: softmax, a row per thread, warps 0-3 the even tiles and 4-7 the odd
+// ones.  Registers: they hold a row of a tile; 2 x 128 threads of 216 and 128 of
+// 72 are the 384 x 168 that the block is launched with.
+constexpr int PAIR_SOFTMAX = 8;
+constexpr int PAIR_PRODUCER = PAIR_SOFTMAX, PAIR_ISSUER = PAIR_SOFTMAX + 1;
+constexpr int PAIR_THREADS = (PAIR_SOFTMAX + 4) * 32;
 constexpr int PAIR_REGS_SOFTMAX = 216, PAIR_REGS_OTHER = 72;
 static_assert(2 * PAIR_REGS_SOFTMAX + PAIR_REGS_OTHER <= 3 * 168, "register split");
 
-struct PairShared {
+template <int HD> struct PairShared {
     PaRun run;
+    struct {
+        PaWalk<PairPlan<HD>::KT> w;
+    } walk[PAIR_SOFTMAX];
+    PaItem tail[PAIR_SOFTMAX];
+    AttnArgs args;
     long long red[PAIR_THREADS / 32];
     uint2 m[2][PA_ROWS];        // a row's m after a tile, by turns, with the tile's number + 1
     float half[2][2][PA_ROWS];  // what the two warps of a row tell each other at an item's end
@@ -934,7 +946,7 @@ M27B_DI float max3(float a, float b, float c) {
 M27B_DI bool pair_follow(const uint2 *p, uint32_t tag, float &m, volatile int *abort, int *status) {
     uint2 v;
     const uint32_t at = smem_u32(p);
-    unsigned long long t0 = 0;
+    uint32_t t0 = 0;
     bool here = true;
     for (unsigned it = 1;; ++it) {
         asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
@@ -948,12 +960,24 @@ M27B_DI bool pair_follow(const uint2 *p, uint32_t tag, float &m, volatile int *a
     return __all_sync(0xffffffffu, here) != 0;
 }
 
+// pa_write for a pair's thread, out of line: inlined, its state costs the tile
+// loop 100 spilled registers a tile.
+template <int HD, bool BF>
+__device__ __noinline__ void pair_write(const AttnArgs &a, const PaWalk<PairPlan<HD>::KT> &w, const PaRun &run, int tok, int rows,
+                                        bool any, float m, float l, uint32_t o, PaItem *tail) {
+    const int warp = threadIdx.x >> 5, row = 32 * (warp & 3) + (threadIdx.x & 31);
+    PaItem t = *tail;
+    __syncwarp();
+    pa_write<HD, BF, 2>(a, w, run, blockIdx.x >> 1, blockIdx.x, tok, a.n_q / a.kv.n_kv, rows, row, warp >> 2, any, m, l, o, t);
+    if ((threadIdx.x & 31) == 0) *tail = t;
+}
+
 template <int HD, bool BF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     k_paged_attn_pair(const AttnArgs a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                       const __grid_constant__ CUtensorMap tmq) {
     using L = PairPlan<HD>;
-    constexpr int KT = L::KT, NS = L::SLOTS, SLOT = L::SLOT, NB = L::NB, WARPS = 2 * PA_SOFTMAX;
+    constexpr int KT = L::KT, NS = L::SLOTS, SLOT = L::SLOT, NB = L::NB;
     extern __shared__ uint8_t pa_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)pa_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = smem + L::Q_BYTES;
@@ -964,32 +988,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     // the second CTA's softmax warps that a tile's V is there
     uint64_t *full = bars, *empty = full + NS, *qfull = empty + NS, *qempty = qfull + 1, *vlanded = qempty + 1, *sfull = vlanded + 2, *sfree = sfull + 2, *pfull = sfree + 2, *pdone = pfull + 2,
              *oread = pdone + 2, *drain = oread + 1, *pair = drain + 1;
-    __shared__ PairShared sh;
+    __shared__ PairShared<HD> sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x & 1, me = blockIdx.x >> 1;
     const int G = a.n_q / a.kv.n_kv, tq = PA_ROWS / G, tqw = 2 * tq;  // tokens of a CTA's rows, of an item
     volatile int *abort = &sh.abort;
 
-    if (warp == PA_PRODUCER) {
+    if (warp == PAIR_PRODUCER) {
         for (int s = lane; s < 2 * NS; s += 32) mbar_init(&full[s], 1);
         if (lane < 4) mbar_init(&pair[lane], 2);
         if (lane < 2) {
             mbar_init(&sfull[lane], 1);
             mbar_init(&vlanded[lane], 1);
-            mbar_init(&sfree[lane], WARPS / 2);
-            mbar_init(&pfull[lane], WARPS / 2);
+            mbar_init(&sfree[lane], PAIR_SOFTMAX);
+            mbar_init(&pfull[lane], PAIR_SOFTMAX);
             mbar_init(&pdone[lane], 1);
         }
         if (lane == 0) {
             mbar_init(qfull, 1);
             mbar_init(qempty, 1);
-            mbar_init(oread, WARPS);
+            mbar_init(oread, 2 * PAIR_SOFTMAX);
             mbar_init(drain, 1);
             sh.abort = 0;
         }
         fence_mbar_init();
     }
-    if (warp == PA_ISSUER) pair_tmem_alloc(&sh.tmem);
+    if (warp == PAIR_ISSUER) pair_tmem_alloc(&sh.tmem);
+    if (tid == 0) sh.args = a;
     if (tid < 2 * PA_ROWS) sh.m[tid >> 7][tid & 127].y = 0;
     pdl_wait();
     pdl_trigger();
@@ -998,11 +1023,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     pair_barrier();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    PaWalk<KT> w(a, sh.run, tqw);
     auto fewer_registers = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_OTHER)); };
 
-    if (warp == PA_PRODUCER) {
+    if (warp == PAIR_PRODUCER) {
         fewer_registers();
+        PaWalk<KT> w;
+        w.begin(a, sh.run, tqw);
         const int ps = a.kv.page_size, shift = 31 - __clz(ps);
         // lane = box: (64-value column, page) of a K slot or a V slot
         const int krows = min(ps, L::KR), knp = L::KR / krows, vrows = min(ps, KT), vnp = KT / vrows;
@@ -1011,7 +1037,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         const uint32_t kdst = kch * (L::KR * 128) + kpg * krows * 128, vdst = vch * (KT * 128) + vpg * vrows * 128;
         int g = 0, item = 0;
         bool ok = true;
-        for (; ok && w.more(); w.next()) {
+        for (; ok && w.more(); w.next(a)) {
             const int n = w.tiles();
             if (n == 0) continue;
             const int *ids = a.kv.table + (long long)w.s.row * a.kv.n_cols;
@@ -1057,7 +1083,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             if (item > 0) mbar_wait_bounded(qfull, (uint32_t)((item - 1) & 1), a.status, 5);
             for (int i = max(0, g - NS); i < g; ++i) mbar_wait_bounded(&full[i % NS], (uint32_t)((i / NS) & 1), a.status, 5);
         }
-    } else if (warp == PA_ISSUER) {
+    } else if (warp == PAIR_ISSUER) {
         fewer_registers();
         if (rank == 0) {
             // The warp stays together and one lane issues; its code is kept
@@ -1069,6 +1095,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                            qdesc = umma_desc128(smem_u32(smem), 16);
             const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), sfull0 = smem_u32(sfull), sfree0 = smem_u32(sfree),
                            pfull0 = smem_u32(pfull), pdone0 = smem_u32(pdone);
+            PaWalk<KT> w;
+            w.begin(a, sh.run, tqw);
             uint32_t t = 0, slot = 0, phase = 0, item = 0;  // t: tile of the next scores; phase: of the slot
             bool ok = true;
             auto used = [&] {
@@ -1078,7 +1106,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             auto wait = [&](uint32_t bar, uint32_t parity) {
                 return ok = __all_sync(0xffffffffu, pa_wait_at(bar, parity, abort, a.status)) != 0;
             };
-            for (; ok && w.more(); w.next()) {
+            for (; ok && w.more(); w.next(a)) {
                 const int n = __shfl_sync(0xffffffffu, w.tiles(), 0);
                 if (n == 0) continue;
                 if (!wait(smem_u32(qfull), item & 1)) break;
@@ -1126,7 +1154,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         // (the second CTA: the first one's last arrival here)
         mbar_wait_bounded(drain, 0u, a.status, 5);
         __syncwarp();
-    } else if (warp >= PA_SOFTMAX) {
+    } else if (warp >= PAIR_SOFTMAX) {
         fewer_registers();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_SOFTMAX));
@@ -1134,9 +1162,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         const int quarter = warp & 3, wg = warp >> 2, row = 32 * quarter + lane;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
         const float c = a.scale * 1.44269504088896340736f;  // log2 e
-        int t0 = 0, g0 = 0, u0 = 0, told = 0, zeroed = 0;  // u0: tiles of this quarter so far (of items where it has live rows)
+        int t0 = 0, u0 = 0, told = 0, zeroed = 0;  // u0: tiles of this quarter so far (of items where it has live rows)
         bool ok = true;
-        PaItem tail = {0, 0, 0, 0};
+        if (lane == 0) sh.tail[warp] = PaItem{0, 0, 0, 0};
         // m after tile u of this quarter, from the warp that has the tile to the
         // other: a word with its tile's number, so that no barrier is needed
         auto publish = [&](int u, float m) {
@@ -1149,16 +1177,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             if (rank == 0) mbar_arrive(bar);
             else pair_arrive(bar);
         };
-        for (; ok && w.more(); w.next()) {
-            const int n = w.tiles(), i0 = w.r * tqw + rank * tq, i = i0 + row / G;
-            const int rows = max(0, min(tq, w.s.q_n - i0)) * G;
+        // the walk's state is in shared memory, for registers' sake
+        PaWalk<KT> &w = sh.walk[warp].w;
+        if (lane == 0) w.begin(a, sh.run, tqw);
+        __syncwarp();
+        while (ok && w.more()) {
+            const int n = w.tiles(), x_first = w.first() * KT, sp_lo = w.sp.lo, sp_hi = w.sp.hi;
+            const int i0 = w.r * tqw + rank * tq, rows = max(0, min(tq, w.s.q_n - i0)) * G;
             const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
             // a dead row's scores are garbage that no one reads
-            const int hi = live ? w.s.base + i + 1 : 0x7fffffff;
+            const int hi = live ? w.s.base + i0 + row / G + 1 : 0x7fffffff;
             const int lo = live && a.window > 0 ? max(0, hi - a.window) : 0;
             float m = -INFINITY, l = 0.0f;  // m in units of c s; l of this warp's tiles
             for (int k = (wg ^ t0) & 1; k < n; k += 2) {
-                const int t = t0 + k, x0 = (w.first() + k) * KT;
+                const int t = t0 + k, x0 = x_first + k * KT;
                 if (!(ok = pa_warp_wait(&sfull[wg], (uint32_t)((t >> 1) & 1), abort, a.status))) break;
                 if (idle) {
                     if (lane == 0) arrive(&sfree[wg]);
@@ -1198,13 +1230,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                         tc_fence_after();
                         const float f = before == -INFINITY ? 1.0f : ex2(before - now);
 #pragma unroll 1
-                        for (int x = 0; x < HD / 32; ++x) {
-                            uint32_t v[32];
-                            tmem_ld32(lane_base + L::O + 32 * x, v);
+                        for (int x = 0; x < HD / 16; ++x) {
+                            uint32_t v[16];
+                            tmem_ld16(lane_base + L::O + 16 * x, v);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                            tmem_st32(lane_base + L::O + 32 * x, v);
+                            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                            tmem_st16(lane_base + L::O + 16 * x, v);
                         }
                         tmem_wait_st();
                     }
@@ -1229,8 +1261,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     l += both.x + both.y;
                 }
                 // values of positions that no row of the item sees
-                if (x0 < w.sp.lo || x0 + KT > w.sp.hi) {
-                    const int g = g0 + min(n, k + 1 + NB) + k;  // V's slot: after K of NB tiles more
+                if (x0 < sp_lo || x0 + KT > sp_hi) {
+                    const int g = 2 * t0 + min(n, k + 1 + NB) + k;  // V's slot: after K of NB tiles more
                     // the first CTA sees the copies of both land, and tells the
                     // second; not before tile t - 2 is done with in both, so
                     // that what it tells is not overtaken
@@ -1242,7 +1274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     uint8_t *v = ring + (size_t)(g % NS) * SLOT;
                     for (int e = tid & 127; e < SLOT / 16; e += 128) {
                         const int x = (e >> 3) % KT;
-                        if (x0 + x < w.sp.lo || x0 + x >= w.sp.hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
+                        if (x0 + x < sp_lo || x0 + x >= sp_hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async();
                     if (rank == 1) asm volatile("fence.acq_rel.cluster;" ::: "memory");
@@ -1273,20 +1305,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     u0 += n;
                 }
             }
-            pa_write<HD, BF>(a, w, sh.run, me, blockIdx.x, w.s.q_lo + i0, G, rows, row, wg, n > 0, m, l, lane_base + L::O, tail);
+            pair_write<HD, BF>(sh.args, w, sh.run, w.s.q_lo + i0, rows, n > 0, m, l, lane_base + L::O, &sh.tail[warp]);
             if (n > 0) {
                 __syncwarp();
                 if (lane == 0) arrive(oread);
             }
             t0 += n;
-            g0 += 2 * n;
+            __syncwarp();
+            if (lane == 0) w.next(a);
+            __syncwarp();
         }
-        if (tid == 0) a.items[blockIdx.x] = tail;
+        if (tid == 0) a.items[blockIdx.x] = sh.tail[0];
     }
     __syncwarp();
     tc_fence_before();
     pair_barrier();
-    if (warp == PA_ISSUER) {
+    if (warp == PAIR_ISSUER) {
         __syncwarp();
         tc_fence_after();
         pair_tmem_free(tmem);
