@@ -789,9 +789,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     if (lane == 0) mbar_arrive(sfree);
                     const int xh = x0 + half * KH;
                     if (__any_sync(0xffffffffu, xh < lo || xh + KH > hi)) {
+                        const uint32_t off = (uint32_t)(xh - lo), len = (uint32_t)max(0, hi - lo);
 #pragma unroll
                         for (int x = 0; x < KH; ++x)
-                            if (xh + x < lo || xh + x >= hi) s[x] = -INFINITY;
+                            if (off + x >= len) s[x] = -INFINITY;
                     }
                     float tops[4] = {s[0], s[1], s[2], s[3]}, theirs;
 #pragma unroll
@@ -887,6 +888,7 @@ template <int HD> struct PairPlan {
     static constexpr int Q_BYTES = PA_ROWS * HD * 2;
     static constexpr int SLOTS = (192 * 1024 - Q_BYTES) / SLOT;
     static constexpr int NB = HD == 256 ? 1 : 2;     // buffers of S
+    static constexpr int AHEAD = 2;                  // products Q K issued ahead of P V
     static constexpr int O = 0, S = HD, P = S + NB * KT;  // TMEM columns: O | S (, S) | P, P
     static constexpr size_t SMEM = 1024 + Q_BYTES + (size_t)SLOTS * SLOT + 1024;
     static_assert(P + KT <= 512, "TMEM plan");
@@ -977,7 +979,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     k_paged_attn_pair(const AttnArgs a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                       const __grid_constant__ CUtensorMap tmq) {
     using L = PairPlan<HD>;
-    constexpr int KT = L::KT, NS = L::SLOTS, SLOT = L::SLOT, NB = L::NB;
+    constexpr int KT = L::KT, NS = L::SLOTS, SLOT = L::SLOT, NB = L::NB, AHEAD = L::AHEAD;
     extern __shared__ uint8_t pa_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)pa_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = smem + L::Q_BYTES;
@@ -1043,12 +1045,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             const int *ids = a.kv.table + (long long)w.s.row * a.kv.n_cols;
             int have = -32, cur = 0;  // lane's page id of page have + lane of the sequence
             auto page_of = [&](int p) { return __shfl_sync(0xffffffffu, cur, (p - have) & 31); };
-            for (int i = 0; ok && i < n + NB; ++i) {
+            for (int i = 0; ok && i < n + AHEAD; ++i) {
                 if (i < n) {
                     const int x0 = (w.first() + i) * KT, plast = (x0 + KT - 1) >> shift;
                     if (plast >= have + 32) {
-                        // from NB tiles before on: that V comes after this K
-                        have = max(0, x0 - NB * KT) >> shift;
+                        // from AHEAD tiles before on: that V comes after this K
+                        have = max(0, x0 - AHEAD * KT) >> shift;
                         cur = pa_page(a, w, ids, have + lane, shift);
                     }
                     const int s = g % NS, xk = x0 + rank * L::KR, page = page_of((xk >> shift) + kpg);
@@ -1067,8 +1069,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                                      w.s.q_lo + w.r * tqw + rank * tq, pair_bar(qfull, 0));
                     ++item;
                 }
-                if (i >= NB) {
-                    const int x0 = (w.first() + i - NB) * KT, s = g % NS, page = page_of((x0 >> shift) + vpg);
+                if (i >= AHEAD) {
+                    const int x0 = (w.first() + i - AHEAD) * KT, s = g % NS, page = page_of((x0 >> shift) + vpg);
                     if (g >= NS && !(ok = pa_warp_wait(&empty[s], (uint32_t)((g / NS - 1) & 1), abort, a.status))) break;
                     if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&full[s], 2 * SLOT);
                     if (vch < L::VC / 64)
@@ -1110,8 +1112,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 const int n = __shfl_sync(0xffffffffu, w.tiles(), 0);
                 if (n == 0) continue;
                 if (!wait(smem_u32(qfull), item & 1)) break;
-                // NB products of Q and K ahead of P V: the scores that the softmax warps will want next
-                for (int i = 0; i < n + NB; ++i) {
+                // Q K runs ahead of P V, which waits for the softmax
+                for (int i = 0; i < n + AHEAD; ++i) {
                     if (i < n) {
                         // S of tile t, once its buffer has been read and the keys are there
                         const uint32_t u = t - NB;
@@ -1129,12 +1131,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                         if (i + 1 == n) pair_commit(lead, smem_u32(qempty));
                         ++t;
                     }
-                    if (i < NB) continue;
-                    const uint32_t v = t - 1 - (i < n ? NB : n + NB - 1 - i);
+                    if (i < AHEAD) continue;
+                    const uint32_t v = t - 1 - (i < n ? AHEAD : n + AHEAD - 1 - i);
                     if (!wait(pfull0 + 8 * (v & 1), (v >> 1) & 1)) break;
                     if (!wait(full0 + 8 * slot, phase)) break;
                     // O of the item before has been read
-                    if (i == NB && item > 0 && !wait(smem_u32(oread), (item - 1) & 1)) break;
+                    if (i == AHEAD && item > 0 && !wait(smem_u32(oread), (item - 1) & 1)) break;
                     tc_fence_after();
                     uint64_t vd = vdesc + (uint64_t)(slot * (SLOT / 16));
                     uint32_t pc = tm + L::P + (v & 1) * (KT / 2);
@@ -1142,7 +1144,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     for (int half = 0; half < 2; ++half, vd += 4 * 128, pc += 32)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            pair_mma_ts(lead, tm + L::O, pc + 8 * kk, vd + 128 * kk, id_o, i > NB || half > 0 || kk > 0);
+                            pair_mma_ts(lead, tm + L::O, pc + 8 * kk, vd + 128 * kk, id_o, i > AHEAD || half > 0 || kk > 0);
                     used();
                     pair_commit(lead, pdone0 + 8 * (v & 1));
                 }
@@ -1204,9 +1206,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) arrive(&sfree[wg]);
                     if (__any_sync(0xffffffffu, x0 < lo || x0 + KT > hi)) {
+                        const uint32_t off = (uint32_t)(x0 - lo), len = (uint32_t)max(0, hi - lo);
 #pragma unroll
                         for (int x = 0; x < KT; ++x)
-                            if (x0 + x < lo || x0 + x >= hi) s[x] = -INFINITY;
+                            if (off + x >= len) s[x] = -INFINITY;
                     }
                     float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -1262,7 +1265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 }
                 // values of positions that no row of the item sees
                 if (x0 < sp_lo || x0 + KT > sp_hi) {
-                    const int g = 2 * t0 + min(n, k + 1 + NB) + k;  // V's slot: after K of NB tiles more
+                    const int g = 2 * t0 + min(n, k + 1 + AHEAD) + k;  // V's slot: after K of AHEAD tiles more
                     // the first CTA sees the copies of both land, and tells the
                     // second; not before tile t - 2 is done with in both, so
                     // that what it tells is not overtaken
