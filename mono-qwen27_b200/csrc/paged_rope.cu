@@ -6,12 +6,13 @@
 //   the head, (c, s) = the position's table entry; q to q_out, k to its slot
 //   of the cache, v to its slot as it is; one rounding to 16 bits at the end.
 //
-// A warp takes one head of one token: lane l holds its values [l V, l V + V),
-// V = head_dim / 32, so the mean is one butterfly, and the second value of a
-// half-layout pair lies n_rot / 2 values, a whole number of lanes, away.
+// A warp has whole heads: lane l holds values [l V, l V + V), V = head_dim / 32,
+// so the mean is one butterfly, and the second value of a half-layout pair
+// lies n_rot / 2 values, a whole number of lanes, away.
 // Bounded by the bytes: each projection value is read once and written once
 // in 16 bits; the table (256 bytes a token at n_rot = 64) stays in L2.
 #include "paged_common.cuh"
+#include "qmv_blk.cuh"
 
 namespace m27b {
 
@@ -24,6 +25,10 @@ struct RopeArgs {
     long long q_out_stride;
     int *status;
 };
+
+M27B_DI void mbar_arrive_local(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 // Sequence of token t: the number of ends cu_q[1..n] at or before t (n: none).
 // 32 probes a step.
@@ -72,6 +77,40 @@ M27B_DI void load_head(const void *base, long long off, float (&x)[V]) {
     }
 }
 
+// The same from shared memory.
+template <bool F32, bool BF, int V>
+M27B_DI void load_head_smem(const uint8_t *base, int d0, float (&x)[V]) {
+    if constexpr (F32) {
+        const float *p = (const float *)base + d0;
+#pragma unroll
+        for (int c = 0; c < V / 2; ++c) {
+            if constexpr (V == 2) {
+                const float2 t = *(const float2 *)p;
+                x[0] = t.x, x[1] = t.y;
+            } else if (c % 2 == 0) {
+                const float4 t = *((const float4 *)p + c / 2);
+                x[2 * c] = t.x, x[2 * c + 1] = t.y, x[2 * c + 2] = t.z, x[2 * c + 3] = t.w;
+            }
+        }
+    } else {
+        uint32_t w[V / 2];
+        const uint16_t *p = (const uint16_t *)base + d0;
+        if constexpr (V == 2) w[0] = *(const uint32_t *)p;
+        else if constexpr (V == 4) {
+            const uint2 t = *(const uint2 *)p;
+            w[0] = t.x, w[1] = t.y;
+        } else {
+            const uint4 t = *(const uint4 *)p;
+            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+        }
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = Half16<BF>::up(w[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+}
+
 template <bool BF, int V>
 M27B_DI void store_head(void *base, long long off, const float (&x)[V]) {
     uint32_t w[V / 2];
@@ -83,84 +122,271 @@ M27B_DI void store_head(void *base, long long off, const float (&x)[V]) {
     else *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// A token's sequence, slot and rotary position; false (and a report) if it has none.
+struct RopeToken {
+    long long slot;  // values from the pools' start to the token's first kv head
+    int rp;
+};
+M27B_DI bool rope_token(const RopeArgs &a, int t, int b, bool report, RopeToken &k) {
+    if (b >= a.bt.n_seq || t < __ldg(a.bt.cu_q + b)) return false;  // of no sequence
+    const int row = seq_row(a.bt, b, a.kv.n_rows);
+    const int p = row < 0 ? -1 : __ldg(a.bt.lens + row) - __ldg(a.bt.cu_q + b + 1) + t;
+    k.rp = a.rope.positions ? __ldg(a.rope.positions + t) : p;
+    const int pc = p / a.kv.page_size;
+    const int page = p >= 0 && pc < a.kv.n_cols ? __ldg(a.kv.table + (long long)row * a.kv.n_cols + pc) : -1;
+    if (page < 0 || page >= a.kv.n_pages || k.rp < 0 || k.rp >= a.rope.n_pos) {
+        if (report) paged_bad(a.status);
+        return false;
+    }
+    k.slot = page * a.kv.page_stride + (long long)(p - pc * a.kv.page_size) * a.kv.n_kv * a.kv.head_dim;
+    return true;
+}
+
+// This lane's cos and sin, from the position's row of the table: pairs d0 / 2 ..
+// (interleaved) or d0 mod (n_rot / 2) .. of lanes that turn.
+template <int V>
+M27B_DI void rope_factors(const RopeArgs &a, const float2 *tab, int d0, float2 (&cs)[V]) {
+    const int half = a.rope.n_rot / 2;
+    if (d0 >= a.rope.n_rot) return;
+    const float4 *at = (const float4 *)(tab + (a.rope.interleaved ? d0 / 2 : d0 < half ? d0 : d0 - half));
+    const int n = a.rope.interleaved ? V / 2 : V;
+    if constexpr (V == 2) {
+        cs[0] = *(const float2 *)at;
+        if (n == 2) cs[1] = *((const float2 *)at + 1);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            if (2 * i < n) {
+                const float4 y = at[i];
+                cs[2 * i] = make_float2(y.x, y.y), cs[2 * i + 1] = make_float2(y.z, y.w);
+            }
+    }
+}
+
+// V consecutive fp32 of norm weights.
+template <int V>
+M27B_DI void norm_weights(const float *w, int d0, float (&v)[V]) {
+    if constexpr (V == 2) {
+        const float2 y = __ldg((const float2 *)(w + d0));
+        v[0] = y.x, v[1] = y.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float4 y = __ldg((const float4 *)(w + d0) + i);
+            v[4 * i] = y.x, v[4 * i + 1] = y.y, v[4 * i + 2] = y.z, v[4 * i + 3] = y.w;
+        }
+    }
+}
+
+// One head of a token: x (this lane's values) normalised and turned.
+template <int V>
+M27B_DI void norm_turn(const RopeArgs &a, bool norm, const float (&nw)[V], const float2 (&cs)[V], int d0, int lane, float (&x)[V]) {
+    if (norm) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss = fmaf(x[i], x[i], ss);
+        const float sc = 1.0f / sqrtf(warp_sum(ss) / (float)(32 * V) + a.h.eps);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = x[i] * sc * nw[i];
+    }
+    const bool turns = d0 < a.rope.n_rot;
+    if (a.rope.interleaved) {
+        if (turns)
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float u = x[2 * i], v = x[2 * i + 1];
+                x[2 * i] = u * cs[i].x - v * cs[i].y;
+                x[2 * i + 1] = u * cs[i].y + v * cs[i].x;
+            }
+    } else {
+        const int half = a.rope.n_rot / 2, dl = half / V;  // lanes between the two values of a pair
+        const bool first = d0 < half;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], first ? lane + dl : lane - dl);
+        if (turns)
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = first ? x[i] * cs[i].x - o[i] * cs[i].y : o[i] * cs[i].y + x[i] * cs[i].x;
+    }
+}
+
+// Few tokens: a warp takes one head of one token.  Its loads go out before the
+// token's sequence, page and slot are looked up (four dependent reads).
 template <bool F32, bool BF, int V>
 __global__ void __launch_bounds__(256) k_rope_append(const RopeArgs a) {
     constexpr int HD = 32 * V;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const int n_rows = a.h.n_q + 2 * a.kv.n_kv;
+    const int lane = threadIdx.x & 31, d0 = lane * V;
+    const int rows = a.h.n_q + 2 * a.kv.n_kv;
     const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const long long t64 = w / n_rows;
+    const long long t64 = w / rows;
     if (t64 >= a.bt.n_tok) return;
-    const int t = (int)t64, r = (int)(w - t64 * n_rows);
-    const int b = find_seq(a.bt.cu_q, a.bt.n_seq, t, lane);
-    if (b >= a.bt.n_seq || t < __ldg(a.bt.cu_q + b)) return;
-    const int row = seq_row(a.bt, b, a.kv.n_rows);
-    const int p = row < 0 ? -1 : __ldg(a.bt.lens + row) - __ldg(a.bt.cu_q + b + 1) + t;
-    const int rp = a.rope.positions ? __ldg(a.rope.positions + t) : p;
-    const int pc = p / a.kv.page_size;
-    const int page = p >= 0 && pc < a.kv.n_cols ? __ldg(a.kv.table + (long long)row * a.kv.n_cols + pc) : -1;
-    if (page < 0 || page >= a.kv.n_pages || rp < 0 || rp >= a.rope.n_pos) {
-        if (lane == 0) paged_bad(a.status);
+    const int t = (int)t64, r = (int)(w - t64 * rows), j = r - a.h.n_q;
+    float x[V], nw[V];
+    const float *norm = r < a.h.n_q ? a.h.q_norm : j < a.kv.n_kv ? a.h.k_norm : nullptr;
+    if (r < a.h.n_q) load_head<F32, BF>(a.h.q, t * a.h.q_stride + (long long)r * HD + d0, x);
+    else if (j < a.kv.n_kv) load_head<F32, BF>(a.h.k, t * a.h.k_stride + (long long)j * HD + d0, x);
+    else load_head<F32, BF>(a.h.v, t * a.h.v_stride + (long long)(j - a.kv.n_kv) * HD + d0, x);
+    if (norm) norm_weights<V>(norm, d0, nw);
+    RopeToken k;
+    if (!rope_token(a, t, find_seq(a.bt.cu_q, a.bt.n_seq, t, lane), lane == 0, k)) return;
+    if (j >= a.kv.n_kv) {
+        store_head<BF>(a.kv.v, k.slot + (long long)(j - a.kv.n_kv) * HD + d0, x);
         return;
     }
-    const long long slot = page * a.kv.page_stride + (long long)(p - pc * a.kv.page_size) * a.kv.n_kv * HD;
-    float x[V];
-    if (r >= a.h.n_q + a.kv.n_kv) {
-        const int j = r - a.h.n_q - a.kv.n_kv;
-        load_head<F32, BF>(a.h.v, t * a.h.v_stride + j * HD + lane * V, x);
-        store_head<BF>(a.kv.v, slot + j * HD + lane * V, x);
+    float2 cs[V];
+    rope_factors<V>(a, (const float2 *)a.rope.table + (long long)k.rp * (a.rope.n_rot / 2), d0, cs);
+    norm_turn<V>(a, norm != nullptr, nw, cs, d0, lane, x);
+    if (r < a.h.n_q) store_head<BF>(a.q_out, t * a.q_out_stride + (long long)r * HD + d0, x);
+    else store_head<BF>(a.kv.k, k.slot + (long long)j * HD + d0, x);
+}
+
+// Many tokens: a unit is up to `per` heads of a token, at most 32 KB of
+// projections.  A producer warp looks the units' tokens up, 32 at a time, and
+// keeps ROPE_STAGES units in flight in shared memory (bulk copies of the unit's
+// q, k and v heads and of the position's row of the table); eight warps turn
+// them.  The lookups' and the memory's latency, which held the kernel above to
+// half of the bandwidth however its warps were sized (9.6k tokens of 32 heads
+// of 256 fp32 values: 85 us, floor 43), are then off the warps' path.
+constexpr int ROPE_STAGES = 3, ROPE_WARPS = 8;
+constexpr int ROPE_STAGE = 32 * 1024, ROPE_TAB = 1024;
+constexpr int ROPE_THREADS = (ROPE_WARPS + 1) * 32;
+constexpr size_t ROPE_SMEM = (size_t)ROPE_STAGES * (ROPE_STAGE + ROPE_TAB);
+
+template <bool F32, bool BF, int V>
+__global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs a, int per, int groups, int wait_code) {
+    constexpr int HD = 32 * V, ES = F32 ? 4 : 2, HB = HD * ES;
+    extern __shared__ __align__(128) uint8_t rope_smem[];
+    __shared__ uint64_t full[ROPE_STAGES], empty[ROPE_STAGES];
+    __shared__ long long slots[ROPE_STAGES];  // the unit's slot; -1: token left out
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d0 = lane * V;
+    const int rows = a.h.n_q + 2 * a.kv.n_kv;
+    const long long units = (long long)a.bt.n_tok * groups, mine = blockIdx.x < units ? (units - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+    uint8_t *tabs = rope_smem + (size_t)ROPE_STAGES * ROPE_STAGE;
+    if (tid == 0) {
+        for (int s = 0; s < ROPE_STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], ROPE_WARPS);
+        }
+        fence_mbar_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    if (warp == ROPE_WARPS) {
+        bool ok = true;
+        RopeToken k = {-1, 0};
+        long long n = 0;
+        for (; ok && n < mine; ++n) {
+            const int s = (int)(n % ROPE_STAGES);
+            if (n % 32 == 0) {
+                // the next 32 units' tokens, one a lane
+                const long long u = blockIdx.x + (n + lane) * (long long)gridDim.x;
+                k.slot = -1;
+                if (n + lane < mine) {
+                    const int t = (int)(u / groups);
+                    int lo = 0, hi = a.bt.n_seq;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) / 2;
+                        if (__ldg(a.bt.cu_q + mid + 1) <= t) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    if (!rope_token(a, t, lo, true, k)) k.slot = -1;
+                }
+                __syncwarp();
+            }
+            const long long slot = __shfl_sync(0xffffffffu, k.slot, (int)(n % 32));
+            const int rp = __shfl_sync(0xffffffffu, k.rp, (int)(n % 32));
+            if (lane == 0) {
+                if (n >= ROPE_STAGES && !mbar_wait_bounded(&empty[s], (uint32_t)((n / ROPE_STAGES - 1) & 1), a.status, wait_code)) ok = false;
+                else {
+                    const long long u = blockIdx.x + n * (long long)gridDim.x;
+                    const int t = (int)(u / groups), r0 = (int)(u - (long long)t * groups) * per, r1 = min(rows, r0 + per);
+                    slots[s] = slot;
+                    if (slot < 0) mbar_arrive_local(&full[s]);
+                    else {
+                        const int nq = max(0, min(r1, a.h.n_q) - r0), kb = a.h.n_q + a.kv.n_kv;
+                        const int k0 = max(r0, a.h.n_q), nk = max(0, min(r1, kb) - k0), v0 = max(r0, kb), nv = max(0, r1 - v0);
+                        uint8_t *st = rope_smem + (size_t)s * ROPE_STAGE;
+                        const uint32_t tb = (uint32_t)a.rope.n_rot * 4;
+                        mbar_arrive_expect_tx(&full[s], (uint32_t)(r1 - r0) * HB + tb);
+                        bulk_copy_g2s(tabs + s * ROPE_TAB, a.rope.table + (long long)rp * a.rope.n_rot, tb, &full[s]);
+                        if (nq) bulk_copy_g2s(st, (const uint8_t *)a.h.q + (t * a.h.q_stride + (long long)r0 * HD) * ES, nq * HB, &full[s]);
+                        if (nk)
+                            bulk_copy_g2s(st + (k0 - r0) * HB, (const uint8_t *)a.h.k + (t * a.h.k_stride + (long long)(k0 - a.h.n_q) * HD) * ES,
+                                          nk * HB, &full[s]);
+                        if (nv)
+                            bulk_copy_g2s(st + (v0 - r0) * HB, (const uint8_t *)a.h.v + (t * a.h.v_stride + (long long)(v0 - kb) * HD) * ES,
+                                          nv * HB, &full[s]);
+                    }
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        }
+        // every copy lands before the shared memory is released (bounded)
+        if (lane == 0)
+            for (long long i = ok ? n : n - 1, e = i; i > 0 && e - i < ROPE_STAGES; --i)
+                mbar_wait_bounded(&full[(i - 1) % ROPE_STAGES], (uint32_t)(((i - 1) / ROPE_STAGES) & 1), a.status, wait_code);
         return;
     }
-    const bool is_q = r < a.h.n_q;
-    const int j = is_q ? r : r - a.h.n_q;
-    load_head<F32, BF>(is_q ? a.h.q : a.h.k, t * (is_q ? a.h.q_stride : a.h.k_stride) + j * HD + lane * V, x);
-    const float *nw = is_q ? a.h.q_norm : a.h.k_norm;
-    if (nw) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss = fmaf(x[i], x[i], ss);
-        const float sc = 1.0f / sqrtf(warp_sum(ss) / (float)HD + a.h.eps);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = x[i] * sc * __ldg(nw + lane * V + i);
-    }
-    const int d0 = lane * V, half = a.rope.n_rot / 2;
-    const float2 *tab = (const float2 *)a.rope.table + (long long)rp * half;
-    if (a.rope.interleaved) {
-        if (d0 < a.rope.n_rot)
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-                const float2 cs = __ldg(tab + d0 / 2 + i);
-                const float u = x[2 * i], v = x[2 * i + 1];
-                x[2 * i] = u * cs.x - v * cs.y;
-                x[2 * i + 1] = u * cs.y + v * cs.x;
+    float qw[V], kw[V];
+    if (a.h.q_norm) norm_weights<V>(a.h.q_norm, d0, qw);
+    if (a.h.k_norm) norm_weights<V>(a.h.k_norm, d0, kw);
+    for (long long n = 0; n < mine; ++n) {
+        const int s = (int)(n % ROPE_STAGES);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (uint32_t)((n / ROPE_STAGES) & 1), a.status, wait_code))) return;
+        const long long u = blockIdx.x + n * (long long)gridDim.x, slot = slots[s];
+        const int t = (int)(u / groups), r0 = (int)(u - (long long)t * groups) * per, r1 = min(rows, r0 + per);
+        if (slot >= 0) {
+            float2 cs[V];
+            rope_factors<V>(a, (const float2 *)(tabs + s * ROPE_TAB), d0, cs);
+            for (int r = r0 + warp; r < r1; r += ROPE_WARPS) {
+                float x[V];
+                load_head_smem<F32, BF>(rope_smem + (size_t)s * ROPE_STAGE + (r - r0) * HB, d0, x);
+                const int j = r - a.h.n_q;
+                if (r < a.h.n_q) {
+                    norm_turn<V>(a, a.h.q_norm != nullptr, qw, cs, d0, lane, x);
+                    store_head<BF>(a.q_out, t * a.q_out_stride + (long long)r * HD + d0, x);
+                } else if (j < a.kv.n_kv) {
+                    norm_turn<V>(a, a.h.k_norm != nullptr, kw, cs, d0, lane, x);
+                    store_head<BF>(a.kv.k, slot + (long long)j * HD + d0, x);
+                } else store_head<BF>(a.kv.v, slot + (long long)(j - a.kv.n_kv) * HD + d0, x);
             }
-    } else {
-        const int dl = half / V;  // lanes between the two values of a pair
-        const bool first = d0 < half;
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], first ? lane + dl : lane - dl);
-        if (d0 < a.rope.n_rot)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float2 cs = __ldg(tab + (first ? d0 : d0 - half) + i);
-                x[i] = first ? x[i] * cs.x - o[i] * cs.y : o[i] * cs.y + x[i] * cs.x;
-            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_local(&empty[s]);
     }
-    if (is_q) store_head<BF>(a.q_out, t * a.q_out_stride + j * HD + d0, x);
-    else store_head<BF>(a.kv.k, slot + j * HD + d0, x);
+}
+
+template <bool F32, bool BF, int V>
+cudaError_t rope_launch_v(const RopeArgs &a, cudaStream_t st) {
+    const int rows = a.h.n_q + 2 * a.kv.n_kv, hb = 32 * V * (F32 ? 4 : 2);
+    const int per = ROPE_STAGE / hb < rows ? ROPE_STAGE / hb : rows, groups = (rows + per - 1) / per;
+    const long long units = (long long)a.bt.n_tok * groups, ctas = 2 * 148;
+    // the stream once every CTA's stages fill twice over
+    if (units >= ctas * 2 * ROPE_STAGES) {
+        static bool ready[64] = {};
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 0 || dev >= 64 || !ready[dev]) {
+            e = cudaFuncSetAttribute(k_rope_stream<F32, BF, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ROPE_SMEM);
+            if (e != cudaSuccess) return e;
+            if (dev >= 0 && dev < 64) ready[dev] = true;
+        }
+        return launch_pdl(k_rope_stream<F32, BF, V>, dim3((unsigned)ctas), dim3(ROPE_THREADS), ROPE_SMEM, st, a, per, groups, 5);
+    }
+    const dim3 grid((unsigned)(((long long)a.bt.n_tok * rows + 7) / 8)), block(256);
+    return launch_pdl(k_rope_append<F32, BF, V>, grid, block, 0, st, a);
 }
 
 template <bool F32, bool BF>
 cudaError_t rope_launch(const RopeArgs &a, cudaStream_t st) {
-    const long long warps = (long long)a.bt.n_tok * (a.h.n_q + 2 * a.kv.n_kv);
-    const dim3 grid((unsigned)((warps + 7) / 8)), block(256);
     switch (a.kv.head_dim) {
-    case 64: return launch_pdl(k_rope_append<F32, BF, 2>, grid, block, 0, st, a);
-    case 128: return launch_pdl(k_rope_append<F32, BF, 4>, grid, block, 0, st, a);
-    default: return launch_pdl(k_rope_append<F32, BF, 8>, grid, block, 0, st, a);
+    case 64: return rope_launch_v<F32, BF, 2>(a, st);
+    case 128: return rope_launch_v<F32, BF, 4>(a, st);
+    default: return rope_launch_v<F32, BF, 8>(a, st);
     }
 }
 
