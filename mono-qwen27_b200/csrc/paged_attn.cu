@@ -49,9 +49,9 @@
 // was set: weights then stay below 2^8 (fp32 sums, and far from the 16-bit
 // types' limits), and O in TMEM is rescaled on few tiles.
 //
-// Rows of a V tile that the item does not see may hold anything: their weights
-// are 0, but 0 * NaN is not, so the softmax warps overwrite them with zeros in
-// shared memory before the product (the first and last tile of an item only).
+// Rows of a V tile that no row of the sequence sees may hold anything: their
+// weights are 0, but 0 * NaN is not, so the softmax warps overwrite them with
+// zeros in shared memory before the product (the tiles at the ends only).
 //
 // Every wait is bounded (2 s; status 5 and the CTA's abort flag).
 #include <cudaTypedefs.h>
@@ -263,11 +263,22 @@ M27B_DI PaSeq pa_seq(const AttnArgs &a, int b, int tq, bool report) {
     return s;
 }
 
+// Positions [x, y) that some row of the sequence sees; the others may hold anything.
+M27B_DI int2 pa_seen(const PaSeq &s, int window) {
+    return make_int2(window > 0 ? max(0, s.base - window + 1) : 0, max(0, s.base + s.q_n));
+}
+
 // Positions [lo, hi) that row tile r sees, and its key tiles [kt0, kt1).
 struct PaSpan {
     int lo, hi, kt0, kt1;
-    M27B_DI int units() const { return max(1, kt1 - kt0); }
 };
+// Units of an item: its key tiles, and the time between two items (the pipeline
+// drains, O leaves) in tiles.  Without it a worker with many short items runs
+// behind: a decode batch of 64 sequences of 300 to 8192 positions ended after
+// 103 us on the median CTA and 146 us on the last.
+constexpr int PA_EXTRA = 3, PAIR_EXTRA = 5;
+template <int EX>
+M27B_DI int pa_units(const PaSpan &s) { return s.kt1 - s.kt0 + EX; }
 template <int KT>
 M27B_DI PaSpan pa_span(const PaSeq &s, int r, int tq, int window) {
     const int i0 = r * tq, i1 = min(s.q_n, i0 + tq);
@@ -281,12 +292,12 @@ M27B_DI PaSpan pa_span(const PaSeq &s, int r, int tq, int window) {
 
 // Units of one kv head of a sequence, for each lane its own; sequences of many
 // row tiles are summed by the whole warp.
-template <int KT>
+template <int KT, int EX>
 M27B_DI long long pa_head_units(const PaSeq &s, int tq, int window) {
     const int lane = threadIdx.x & 31;
     long long u = 0;
     if (s.nrt <= 4)
-        for (int r = 0; r < s.nrt; ++r) u += pa_span<KT>(s, r, tq, window).units();
+        for (int r = 0; r < s.nrt; ++r) u += pa_units<EX>(pa_span<KT>(s, r, tq, window));
     for (unsigned big = __ballot_sync(0xffffffffu, s.nrt > 4); big; big &= big - 1) {
         const int src = __ffs(big) - 1;
         PaSeq o;
@@ -294,7 +305,7 @@ M27B_DI long long pa_head_units(const PaSeq &s, int tq, int window) {
         o.base = __shfl_sync(0xffffffffu, s.base, src);
         o.nrt = __shfl_sync(0xffffffffu, s.nrt, src);
         long long v = 0;
-        for (int r = lane; r < o.nrt; r += 32) v += pa_span<KT>(o, r, tq, window).units();
+        for (int r = lane; r < o.nrt; r += 32) v += pa_units<EX>(pa_span<KT>(o, r, tq, window));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
         if (lane == src) u = v;
@@ -318,7 +329,7 @@ M27B_DI long long div_count(long long x, long long y) {
 }
 
 // The item at hand, walked alike by every role.
-template <int KT>
+template <int KT, int EX>
 struct PaWalk {
     long long u, end;
     int tq, b, j, r, off;
@@ -334,12 +345,13 @@ struct PaWalk {
     M27B_DI bool more() const { return u < end; }
     M27B_DI void span(const AttnArgs &a) {
         sp = pa_span<KT>(s, r, tq, a.window);
-        take = (int)min((long long)(sp.units() - off), end - u);
+        take = (int)min((long long)(pa_units<EX>(sp) - off), end - u);
     }
     // key tiles of this item in this run
-    M27B_DI int tiles() const { return sp.kt1 > sp.kt0 ? take : 0; }
-    M27B_DI int first() const { return sp.kt0 + off; }
-    M27B_DI bool whole() const { return off == 0 && take == sp.units(); }
+    M27B_DI int tiles() const { return max(0, off + take - EX) - max(0, off - EX); }
+    M27B_DI int first() const { return sp.kt0 + max(0, off - EX); }
+    M27B_DI int units() const { return pa_units<EX>(sp); }
+    M27B_DI bool whole() const { return off == 0 && take == units(); }
     M27B_DI void next(const AttnArgs &a) {
         u += take;
         off = 0;
@@ -379,7 +391,7 @@ M27B_DI long long pa_scan(long long v, long long *red, long long *total) {
 }
 
 // All threads: fill `run` (shared memory) with the run of worker `me` of at most `most`.
-template <int KT>
+template <int KT, int EX>
 M27B_DI void pa_find_run(const AttnArgs &a, int tq, int me, int most, PaRun *run, long long *red) {
     const int n = a.bt.n_seq, nt = blockDim.x;
     long long total = 0, head = 0, u = 0, before = 0, sum;
@@ -388,7 +400,7 @@ M27B_DI void pa_find_run(const AttnArgs &a, int tq, int me, int most, PaRun *run
         const int b = b0 + threadIdx.x;
         s = {0, 0, 0, 0, 0};
         if (b < n) s = pa_seq(a, b, tq, blockIdx.x == 0);
-        head = pa_head_units<KT>(s, tq, a.window);
+        head = pa_head_units<KT, EX>(s, tq, a.window);
         u = head * a.kv.n_kv;
         before = pa_scan(u, red, &sum);
         total += sum;
@@ -408,7 +420,7 @@ M27B_DI void pa_find_run(const AttnArgs &a, int tq, int me, int most, PaRun *run
         if (n > nt) {
             s = {0, 0, 0, 0, 0};
             if (b < n) s = pa_seq(a, b, tq, false);
-            head = pa_head_units<KT>(s, tq, a.window);
+            head = pa_head_units<KT, EX>(s, tq, a.window);
             u = head * a.kv.n_kv;
             before = pa_scan(u, red, &sum);
         }
@@ -428,7 +440,7 @@ M27B_DI void pa_find_run(const AttnArgs &a, int tq, int me, int most, PaRun *run
         long long off = run->seq_off - j * run->head_units;
         int r0 = 0;
         for (;; r0 += 32) {
-            const int v = r0 + lane < s.nrt ? pa_span<KT>(s, r0 + lane, tq, a.window).units() : 0;
+            const int v = r0 + lane < s.nrt ? pa_units<EX>(pa_span<KT>(s, r0 + lane, tq, a.window)) : 0;
             long long inc = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -570,7 +582,7 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
         // the item begins with worker c0 and ends with c1
         const long long U = w.u - w.off;
         const int c0 = (int)div_count((U + 1) * run.workers + run.total - 1, run.total) - 1;
-        const int c1 = (int)div_count((U + w.sp.units()) * run.workers + run.total - 1, run.total) - 1;
+        const int c1 = (int)div_count((U + w.units()) * run.workers + run.total - 1, run.total) - 1;
         if (me == c0) tail = {rows > 0 ? c1 - c0 + 1 : 0, rows, tok, w.j};
         if (idle) return;
         float *rec = a.part + (size_t)(2 * cta + (me == c0 ? 1 : 0)) * pa_record(HD);
@@ -629,11 +641,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     pdl_wait();
     pdl_trigger();
     tc_fence_before();
-    pa_find_run<KT>(a, tq, me, gridDim.x, &sh.run, sh.red);
+    pa_find_run<KT, PA_EXTRA>(a, tq, me, gridDim.x, &sh.run, sh.red);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    PaWalk<KT> w;
+    PaWalk<KT, PA_EXTRA> w;
     w.begin(a, sh.run, tq);
 
     if (warp == PA_PRODUCER) {
@@ -747,7 +759,30 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             theirs = *(volatile float *)&sh.half[turn][half ^ 1][row];
             return here;
         };
-        for (; ok && w.more(); w.next(a)) {
+        // half of the row's Q of an item into TMEM
+        auto load_q = [&](const PaWalk<KT, PA_EXTRA> &x) {
+            const int i = x.r * tq + row / G;
+            const bool live = row < tq * G && i < x.s.q_n;
+            const uint16_t *qp = (const uint16_t *)a.q + (long long)(x.s.q_lo + i) * a.q_stride + (long long)(x.j * G + row % G) * HD +
+                                 half * (HD / 2);
+#pragma unroll
+            for (int y = 0; y < HD / 64; ++y) {
+                uint32_t v[16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint4 z = live ? __ldg((const uint4 *)(qp + 32 * y) + e) : make_uint4(0, 0, 0, 0);
+                    v[4 * e] = z.x, v[4 * e + 1] = z.y, v[4 * e + 2] = z.z, v[4 * e + 3] = z.w;
+                }
+                tmem_st16(lane_base + L::Q + half * (HD / 4) + 16 * y, v);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qfull);
+        };
+        if (w.more() && w.tiles() > 0) load_q(w);
+        while (ok && w.more()) {
+            const int2 seen = pa_seen(w.s, a.window);
             const int n = w.tiles(), i0 = w.r * tq, i = i0 + row / G, h = w.j * G + row % G;
             const int rows = min(tq, w.s.q_n - i0) * G;
             const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
@@ -755,24 +790,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const int hi = live ? w.s.base + i + 1 : 0x7fffffff;
             const int lo = live && a.window > 0 ? max(0, hi - a.window) : 0;
             float m = -INFINITY, l = 0.0f;  // m in units of c s
-            if (n > 0) {
-                // half of this row's Q into TMEM (its last product has been read as S)
-                const uint16_t *qp = (const uint16_t *)a.q + (long long)(w.s.q_lo + i) * a.q_stride + (long long)h * HD + half * (HD / 2);
-#pragma unroll
-                for (int x = 0; x < HD / 64; ++x) {
-                    uint32_t v[16];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint4 y = live ? __ldg((const uint4 *)(qp + 32 * x) + e) : make_uint4(0, 0, 0, 0);
-                        v[4 * e] = y.x, v[4 * e + 1] = y.y, v[4 * e + 2] = y.z, v[4 * e + 3] = y.w;
-                    }
-                    tmem_st16(lane_base + L::Q + half * (HD / 4) + 16 * x, v);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(qfull);
-            }
             for (int k = 0; k < n; ++k, ++t) {
                 const int x0 = (w.first() + k) * KT;
                 if (!(ok = pa_warp_wait(sfull, (uint32_t)(t & 1), abort, a.status))) break;
@@ -838,14 +855,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     if constexpr (KH == 64) tmem_st32(pc, p);
                     else tmem_st16(pc, p);
                 }
-                // values of positions that no row of the item sees
-                if (x0 < w.sp.lo || x0 + KT > w.sp.hi) {
+                // values of positions that no row of the sequence sees
+                if (x0 < seen.x || x0 + KT > seen.y) {
                     const int g = g0 + (k == n - 1 ? 2 * n - 1 : 2 * k + 2);  // V's slot: K0 K1 V0 K2 V1 ...
                     if (!(ok = pa_warp_wait(&full[g % NS], (uint32_t)((g / NS) & 1), abort, a.status))) break;
                     uint8_t *v = ring + (size_t)(g % NS) * SLOT;
                     for (int e = tid; e < SLOT / 16; e += 32 * PA_SOFTMAX) {
                         const int x = (e >> 3) % KT;
-                        if (x0 + x < w.sp.lo || x0 + x >= w.sp.hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
+                        if (x0 + x < seen.x || x0 + x >= seen.y) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async();
                 }
@@ -856,6 +873,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             if (!ok) break;
             g0 += 2 * n;
+            // the next item's Q, while the last product here runs: the products
+            // with this one are done, since their scores have been read
+            PaWalk<KT, PA_EXTRA> next = w;
+            next.next(a);
+            if (next.more() && next.tiles() > 0) load_q(next);
             if (n > 0) {
                 if (!(ok = pa_warp_wait(&pdone[(t - 1) & 1], (uint32_t)(((t - 1) >> 1) & 1), abort, a.status))) break;
                 tc_fence_after();
@@ -866,6 +888,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 l = half ? theirs + l : l + theirs;
             }
             pa_write<HD, BF, 2>(a, w, sh.run, me, blockIdx.x, w.s.q_lo + i0, G, rows, row, half, n > 0, m, l, lane_base + L::O, tail);
+            w = next;
         }
         if (tid == 0) a.items[blockIdx.x] = tail;
     }
@@ -906,7 +929,7 @@ static_assert(2 * PAIR_REGS_SOFTMAX + PAIR_REGS_OTHER <= 3 * 168, "register spli
 template <int HD> struct PairShared {
     PaRun run;
     struct {
-        PaWalk<PairPlan<HD>::KT> w;
+        PaWalk<PairPlan<HD>::KT, PAIR_EXTRA> w;
     } walk[PAIR_SOFTMAX];
     PaItem tail[PAIR_SOFTMAX];
     AttnArgs args;
@@ -965,7 +988,7 @@ M27B_DI bool pair_follow(const uint2 *p, uint32_t tag, float &m, volatile int *a
 // pa_write for a pair's thread, out of line: inlined, its state costs the tile
 // loop 100 spilled registers a tile.
 template <int HD, bool BF>
-__device__ __noinline__ void pair_write(const AttnArgs &a, const PaWalk<PairPlan<HD>::KT> &w, const PaRun &run, int tok, int rows,
+__device__ __noinline__ void pair_write(const AttnArgs &a, const PaWalk<PairPlan<HD>::KT, PAIR_EXTRA> &w, const PaRun &run, int tok, int rows,
                                         bool any, float m, float l, uint32_t o, PaItem *tail) {
     const int warp = threadIdx.x >> 5, row = 32 * (warp & 3) + (threadIdx.x & 31);
     PaItem t = *tail;
@@ -1021,7 +1044,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     pdl_wait();
     pdl_trigger();
     tc_fence_before();
-    pa_find_run<KT>(a, tqw, me, gridDim.x >> 1, &sh.run, sh.red);
+    pa_find_run<KT, PAIR_EXTRA>(a, tqw, me, gridDim.x >> 1, &sh.run, sh.red);
     pair_barrier();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
@@ -1029,7 +1052,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
     if (warp == PAIR_PRODUCER) {
         fewer_registers();
-        PaWalk<KT> w;
+        PaWalk<KT, PAIR_EXTRA> w;
         w.begin(a, sh.run, tqw);
         const int ps = a.kv.page_size, shift = 31 - __clz(ps);
         // lane = box: (64-value column, page) of a K slot or a V slot
@@ -1097,7 +1120,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                            qdesc = umma_desc128(smem_u32(smem), 16);
             const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty), sfull0 = smem_u32(sfull), sfree0 = smem_u32(sfree),
                            pfull0 = smem_u32(pfull), pdone0 = smem_u32(pdone);
-            PaWalk<KT> w;
+            PaWalk<KT, PAIR_EXTRA> w;
             w.begin(a, sh.run, tqw);
             uint32_t t = 0, slot = 0, phase = 0, item = 0;  // t: tile of the next scores; phase: of the slot
             bool ok = true;
@@ -1180,11 +1203,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             else pair_arrive(bar);
         };
         // the walk's state is in shared memory, for registers' sake
-        PaWalk<KT> &w = sh.walk[warp].w;
+        PaWalk<KT, PAIR_EXTRA> &w = sh.walk[warp].w;
         if (lane == 0) w.begin(a, sh.run, tqw);
         __syncwarp();
         while (ok && w.more()) {
-            const int n = w.tiles(), x_first = w.first() * KT, sp_lo = w.sp.lo, sp_hi = w.sp.hi;
+            const int n = w.tiles(), x_first = w.first() * KT;
+            const int2 seen = pa_seen(w.s, a.window);
             const int i0 = w.r * tqw + rank * tq, rows = max(0, min(tq, w.s.q_n - i0)) * G;
             const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
             // a dead row's scores are garbage that no one reads
@@ -1263,8 +1287,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     const float2 both = unpack2(add2(sum[0], sum[1]));
                     l += both.x + both.y;
                 }
-                // values of positions that no row of the item sees
-                if (x0 < sp_lo || x0 + KT > sp_hi) {
+                // values of positions that no row of the sequence sees
+                if (x0 < seen.x || x0 + KT > seen.y) {
                     const int g = 2 * t0 + min(n, k + 1 + AHEAD) + k;  // V's slot: after K of AHEAD tiles more
                     // the first CTA sees the copies of both land, and tells the
                     // second; not before tile t - 2 is done with in both, so
@@ -1277,7 +1301,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     uint8_t *v = ring + (size_t)(g % NS) * SLOT;
                     for (int e = tid & 127; e < SLOT / 16; e += 128) {
                         const int x = (e >> 3) % KT;
-                        if (x0 + x < sp_lo || x0 + x >= sp_hi) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
+                        if (x0 + x < seen.x || x0 + x >= seen.y) *(uint4 *)(v + (size_t)e * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async();
                     if (rank == 1) asm volatile("fence.acq_rel.cluster;" ::: "memory");
@@ -1364,6 +1388,7 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
             for (int v = 0; v < 8; ++v) o[v] *= f0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
+                if (ml[q].x == -INFINITY) continue;  // the part saw nothing (its O may be anything)
                 const float f = ex2(ml[q].x - ref);
                 l = fmaf(f, ml[q].y, l);
 #pragma unroll
@@ -1405,7 +1430,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const AttnArgs a, int stride
     pdl_trigger();
     const PaItem it = a.items[blockIdx.x];
     if (it.np == 0) return;
-    if (it.np <= 2) pa_join<HD, BF, 2>(a, it, stride);
+    if (it.np <= 8) pa_join<HD, BF, 2>(a, it, stride);
     else pa_join<HD, BF, 8>(a, it, stride);
 }
 
