@@ -1425,12 +1425,18 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
 }
 
 template <int HD, bool BF>
-__global__ void __launch_bounds__(256) k_paged_join(const AttnArgs a, int stride) {
+__global__ void __launch_bounds__(256, 4) k_paged_join(const AttnArgs a, int stride) {
     pdl_wait();
     pdl_trigger();
     const PaItem it = a.items[blockIdx.x];
     if (it.np == 0) return;
-    if (it.np <= 8) pa_join<HD, BF, 2>(a, it, stride);
+    // the group size with the fewest round trips: those of a value (four parts
+    // a thread each), times the values of a group
+    const int tasks = it.rows * (HD / 8), threads = 256 * gridDim.y;
+    auto trips = [&](int sp) { return (tasks * sp + threads - 1) / threads * (2 * ((it.np + 4 * sp - 1) / (4 * sp)) + 1); };
+    const int t1 = trips(1), t2 = trips(2), t8 = trips(8);
+    if (t1 <= t2 && t1 <= t8) pa_join<HD, BF, 1>(a, it, stride);
+    else if (t2 <= t8) pa_join<HD, BF, 2>(a, it, stride);
     else pa_join<HD, BF, 8>(a, it, stride);
 }
 
@@ -1498,6 +1504,22 @@ cudaError_t pa_ready(K kern, size_t smem, bool (&done)[64]) {
     return e;
 }
 
+// The join after it.  It asks for the same split of L1 as the kernel before
+// (all shared memory), so that the SMs need not drain to change it.
+template <int HD, bool BF>
+cudaError_t pa_join_launch(const AttnArgs &a, int ctas, int stride, cudaStream_t st) {
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        e = cudaFuncSetAttribute(k_paged_join<HD, BF>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    return launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 8), dim3(256), 0, st, a, stride);
+}
+
 template <int HD, bool BF>
 cudaError_t pa_launch(const AttnArgs &a, int G, bool pair, int ctas, cudaStream_t st, bool *maps) {
     CUtensorMap tk, tv, tq;
@@ -1510,7 +1532,7 @@ cudaError_t pa_launch(const AttnArgs &a, int G, bool pair, int ctas, cudaStream_
             if (!*maps) return cudaSuccess;
             e = pa_ready(k_paged_attn_pair<HD, BF>, L::SMEM, ready);
             if (e == cudaSuccess) e = launch_pdl(k_paged_attn_pair<HD, BF>, dim3(ctas), dim3(PAIR_THREADS), L::SMEM, st, a, tk, tv, tq);
-            return e != cudaSuccess ? e : launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 8), dim3(256), 0, st, a, 2);
+            return e != cudaSuccess ? e : pa_join_launch<HD, BF>(a, ctas, 2, st);
         }
     }
     using L = PaPlan<HD>;
@@ -1519,7 +1541,7 @@ cudaError_t pa_launch(const AttnArgs &a, int G, bool pair, int ctas, cudaStream_
     if (!*maps) return cudaSuccess;
     e = pa_ready(k_paged_attn<HD, BF>, L::SMEM, ready);
     if (e == cudaSuccess) e = launch_pdl(k_paged_attn<HD, BF>, dim3(ctas), dim3(PA_THREADS), L::SMEM, st, a, tk, tv);
-    return e != cudaSuccess ? e : launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 8), dim3(256), 0, st, a, 1);
+    return e != cudaSuccess ? e : pa_join_launch<HD, BF>(a, ctas, 1, st);
 }
 
 template <bool BF>
