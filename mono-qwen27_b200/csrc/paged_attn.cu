@@ -1220,6 +1220,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 if (!(ok = pa_warp_wait(&sfull[wg], (uint32_t)((t >> 1) & 1), abort, a.status))) break;
                 if (idle) {
                     if (lane == 0) arrive(&sfree[wg]);
+                    // as the others before they write P: the scores of t come before
+                    // the product of t - 2 has its P, and an arrival for t must not
+                    // be taken for one for t - 2
+                    if (t >= 2 && !(ok = pa_warp_wait(&pdone[wg], (uint32_t)(((t - 2) >> 1) & 1), abort, a.status))) break;
                 } else {
                     tc_fence_after();
                     float s[KT];

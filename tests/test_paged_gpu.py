@@ -247,9 +247,138 @@ def test_attn_other_stream_and_graph(torch, m27b):
     assert torch.equal(out, want)
 
 
-def test_attn_offsets_past_32_bits(torch, m27b):
+# Batches of many rows a sequence run on pairs of CTAs (head_dim 128 and 256).
+
+
+@pytest.mark.parametrize("ps", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("hd,dtype", [(128, "f16"), (256, "bf16")])
+def test_attn_many_rows_page_sizes(torch, m27b, hd, dtype, ps):
+    _check_attn(torch, m27b, [300, 0, 131, 1], [701, 50, 131, 400], 8, 2, hd, dtype, ps, seed=30)
+
+
+@pytest.mark.parametrize("window", [1, 63, 100, 128, 129, 500])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_attn_many_rows_window(torch, m27b, window, hd):
+    _check_attn(torch, m27b, [260, 170], [900, 170], 6, 2, hd, "bf16", 32, window=window, seed=31)
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(1, 1), (128, 1), (7, 1), (10, 5), (64, 1)])
+def test_attn_many_rows_head_groups(torch, m27b, n_q, n_kv):
+    n = max(3, 600 // (n_q // n_kv))
+    _check_attn(torch, m27b, [n, 2 * n], [n + 150, 2 * n], n_q, n_kv, 128, "bf16", 16, seed=32)
+
+
+def test_attn_many_rows_empty_and_idle(torch, m27b):
+    # fewer positions than tokens, none at all, one token, no tokens
+    _check_attn(torch, m27b, [400, 90, 0, 300, 1], [150, 0, 77, 300, 513], 8, 2, 128, "f16", 16, seed=33)
+    _check_attn(torch, m27b, [257, 3], [100, 0], 12, 2, 256, "bf16", 16, window=40, seed=34)
+
+
+def test_attn_many_rows_split_runs(torch, m27b):
+    # one long item list per kv head: every run begins and ends inside an item
+    _check_attn(torch, m27b, [64], [6000], 4, 1, 256, "bf16", 64, seed=35)
+    _check_attn(torch, m27b, [700], [1500], 4, 2, 128, "f16", 32, seed=36)
+
+
+def test_attn_many_rows_strides_and_rows(torch, m27b):
+    _check_attn(torch, m27b, [140, 100], [340, 100], 6, 2, 256, "f16", 32, seed=37, pad=8, rows=[3, 1], strided=True, scale=0.2)
+    _check_attn(torch, m27b, [200], [333], 8, 2, 128, "bf16", 16, seed=38, pad=64, rows=[2], strided=True)
+
+
+@pytest.mark.parametrize("gain", [0.0, 8.0, 40.0])
+def test_attn_many_rows_flat_and_sharp(torch, m27b, gain):
+    _check_attn(torch, m27b, [200], [777], 6, 2, 128, "bf16", 16, seed=39, q_gain=gain)
+
+
+def test_attn_many_rows_rising_scores(torch, m27b):
+    for hd in (128, 256):
+        n, ps = 900, 16
+        c = Cache(torch, m27b, [n], ps, 1, hd, "bf16", 40)
+        ids = torch.from_numpy(c.tab[0, :P.cdiv(n, ps)].astype(np.int64)).cuda()
+        ramp = torch.arange(len(ids) * ps, device="cuda").view(-1, ps, 1).float() / 900
+        c.k[ids] = ramp[..., None].expand(-1, -1, 1, hd).to(torch.bfloat16)
+        q = torch.ones(160, 2, hd, dtype=torch.bfloat16, device="cuda")
+        out, lse = torch.empty_like(q), torch.empty(160, 2, device="cuda")
+        m27b.paged_attn(c.kv, q, _cu(torch, [160]), c.lens, out, m27b.paged_attn_scratch(2, 1, hd), scale=1.0, lse=lse)
+        o, l, mag, big = P.attend(_np(q), *c.seq(0), 1.0, 0)
+        ds = 2.0 ** -19 * big + 1e-6
+        u = P.U["bf16"]
+        assert (np.abs(_np(out) - o) <= u * np.abs(o) + (u + 2 * ds[..., None]) * mag * 1.02 + 1e-7).all()
+        assert (np.abs(_np(lse) - l) <= ds + 1e-6 * (1 + np.abs(l))).all()
+
+
+def test_attn_many_sequences_of_many_rows(torch, m27b):
+    rng = random.Random(41)
+    q = [rng.choice([0, 2, 3, 4]) for _ in range(500)]
+    _check_attn(torch, m27b, q, [x + rng.randrange(0, 40) for x in q], 128, 1, 128, "f16", 16, seed=42)
+
+
+def test_attn_many_rows_same_every_time_other_stream_graph(torch, m27b):
+    c = Cache(torch, m27b, [1500, 260], 16, 2, 256, "bf16", 43)
+    q = torch.randn(560, 8, 256, device="cuda").bfloat16()
+    cu, scr = _cu(torch, [300, 260]), m27b.paged_attn_scratch(8, 2, 256)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    m27b.paged_attn(c.kv, q, cu, c.lens, want, scr)
+    for _ in range(8):
+        m27b.paged_attn(c.kv, q, cu, c.lens, out, scr)
+        assert torch.equal(out, want)
+    torch.cuda.synchronize()
+    out.zero_()
+    s = torch.cuda.Stream()
+    m27b.paged_attn(c.kv, q, cu, c.lens, out, scr, stream=s)
+    s.synchronize()
+    assert torch.equal(out, want)
+    out.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        m27b.paged_attn(c.kv, q, cu, c.lens, out, scr)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_attn_pages_before_the_window_may_be_gone(torch, m27b):
+    # pages that no row sees: given back (-1) or anything
+    for hd, nq, n_q, n_kv in ((128, 1, 16, 8), (256, 3, 8, 2), (128, 150, 8, 2), (256, 150, 8, 2)):
+        n, ps, window = 900, 16, 100
+        c = Cache(torch, m27b, [n], ps, n_kv, hd, "bf16", 44)
+        first = (n - nq - window + 1) // ps  # the first page of the first row's window
+        tab = c.table.clone()
+        tab[0, :first] = -1
+        tab[0, 0] = 1 << 30
+        q = torch.randn(nq, n_q, hd, device="cuda").bfloat16()
+        out = torch.empty_like(q)
+        k, v = c.seq(0)
+        page = c.tab[0, first]  # slots of the window's first page that no row sees
+        gone = n - nq - window + 1 - first * ps
+        if gone > 0:
+            c.k[int(page), :gone], c.v[int(page), :gone] = float("inf"), float("nan")
+        m27b.paged_attn(m27b.PagedKV(c.k, c.v, tab), q, _cu(torch, [nq]), c.lens, out, m27b.paged_attn_scratch(n_q, n_kv, hd), window=window)
+        o, _, mag, _ = P.attend(_np(q), k, v, hd ** -0.5, window)
+        assert (np.abs(_np(out) - o) <= 2.0 ** -8 * (np.abs(o) + 1.1 * mag) + 1e-6).all()
+        assert m27b.device_status() == 0
+
+
+def test_attn_token_offsets_are_held_to_the_buffers(torch, m27b):
+    # offsets past the last token: what is there is attended, nothing beyond is touched
+    c = Cache(torch, m27b, [50, 60], 16, 2, 64, "bf16", 45)
+    q = torch.randn(4, 4, 64, device="cuda").bfloat16()
+    wide = torch.full((6, 4, 64), 3.0, device="cuda").bfloat16()
+    cu = torch.tensor([0, 2, 9], dtype=torch.int32, device="cuda")
+    m27b.paged_attn(c.kv, q, cu, c.lens, wide[:4], m27b.paged_attn_scratch(4, 2, 64))
+    o, _, mag, _ = P.attend(_np(q)[:2], *c.seq(0), 0.125, 0)
+    assert (np.abs(_np(wide)[:2] - o) <= 2.0 ** -8 * (np.abs(o) + 1.1 * mag) + 1e-6).all()
+    assert (wide[4:] == 3.0).all() and torch.isfinite(wide.float()).all()
+    cu = torch.tensor([3, 1, 2], dtype=torch.int32, device="cuda")  # descending: no tokens
+    wide.fill_(3.0)
+    m27b.paged_attn(c.kv, q, cu, c.lens, wide[:4], m27b.paged_attn_scratch(4, 2, 64))
+    assert (wide[[0, 2, 3]] == 3.0).all()
+
+
+@pytest.mark.parametrize("hd,nq", [(64, 3), (128, 3), (128, 140)])
+def test_attn_offsets_past_32_bits(torch, m27b, hd, nq):
     # pages 2^27 values apart: 40 of them reach past 2^32 values
-    stride, ps, n_kv, hd, n = 1 << 27, 16, 2, 64, 37 * 16 + 5
+    stride, ps, n_kv, n = 1 << 27, 16, 2, 37 * 16 + 5
     k = torch.empty(39 * stride + ps * n_kv * hd, dtype=torch.float16, device="cuda")
     v = torch.empty_like(k)
     kp, vp = (x.as_strided((40, ps, n_kv, hd), (stride, n_kv * hd, hd, 1)) for x in (k, v))
@@ -258,9 +387,9 @@ def test_attn_offsets_past_32_bits(torch, m27b):
         vp[p].normal_()
     table = torch.arange(39, 0, -1, dtype=torch.int32, device="cuda").view(1, -1).contiguous()
     kv = m27b.PagedKV(kp, vp, table)
-    q = torch.randn(3, 4, hd, device="cuda").half()
+    q = torch.randn(nq, 4, hd, device="cuda").half()
     out = torch.empty_like(q)
-    m27b.paged_attn(kv, q, _cu(torch, [3]), torch.tensor([n], dtype=torch.int32, device="cuda"), out,
+    m27b.paged_attn(kv, q, _cu(torch, [nq]), torch.tensor([n], dtype=torch.int32, device="cuda"), out,
                     m27b.paged_attn_scratch(4, n_kv, hd))
     ids = table[0, :38].long()
     o, _, mag, _ = P.attend(_np(q), *(_np(x[ids]).reshape(-1, n_kv, hd)[:n] for x in (kp, vp)), hd ** -0.5, 0)
@@ -324,7 +453,8 @@ def _check_rope(torch, m27b, q_lens, kv_lens, n_q, n_kv, hd, dtype, src, ps, n_r
         same = np.isnan(want) | np.isinf(want)
         assert np.array_equal(got[same], want[same], equal_nan=True)
         big = np.abs(np.where(same, 0, want)).max(-1, keepdims=True)
-        assert (np.abs(got - want) <= u * np.abs(want) + 2e-6 * big + 1e-7)[~same].all()
+        with np.errstate(invalid="ignore"):
+            assert (np.abs(got - want) <= u * np.abs(want) + 2e-6 * big + 1e-7)[~same].all()
     if pad:
         assert torch.isfinite(c.buf[0][:, -pad:].float()).all()
     assert m27b.device_status() == 0
@@ -364,6 +494,31 @@ def test_rope_append_many_sequences(torch, m27b):
     rng = random.Random(25)
     q = [rng.choice([0, 1, 2, 3]) for _ in range(1300)]
     _check_rope(torch, m27b, q, [x + rng.randrange(20) for x in q], 2, 1, 64, "bf16", "f32", 16, 64, False, False, seed=26)
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd,src,dtype,ps", [(2, 1, 64, "f32", "bf16", 16), (40, 8, 256, "f32", "bf16", 64),
+                                                      (16, 8, 128, "f16", "f16", 32), (6, 2, 256, "bf16", "bf16", 128)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_append_many_tokens(torch, m27b, n_q, n_kv, hd, src, dtype, ps, interleaved):
+    # enough tokens for the streaming kernel; 40 + 16 heads of 256 fp32 values are two units a token
+    _check_rope(torch, m27b, [1200, 0, 700], [1200, 5, 1000], n_q, n_kv, hd, dtype, src, ps, hd // 2, interleaved, True, seed=50,
+                rows=[2, 0, 1])
+
+
+def test_rope_append_many_tokens_in_place_and_left_out(torch, m27b):
+    _check_rope(torch, m27b, [1900], [2000], 4, 2, 128, "f16", "f16", 32, 64, True, False, seed=51, in_place=True)
+    # tokens of no sequence, and positions past the table, among many
+    c = Cache(torch, m27b, [1000], 16, 1, 64, "bf16", 52, poison=False)
+    x = torch.randn(3000, 3, 64, device="cuda")
+    q = torch.full((3000, 1, 64), 9.0, device="cuda").bfloat16()
+    k0 = c.k.clone()
+    m27b.rope_append(c.kv, x[:, :1], x[:, 1:2], x[:, 2:], torch.tensor([100, 1100], dtype=torch.int32, device="cuda"), c.lens,
+                     m27b.rope_table(990, 64, 1e4), q)
+    assert m27b.device_status() == 6
+    assert (q[:100] == 9.0).all() and (q[1090:] == 9.0).all() and not (q[100:1090] == 9.0).all(-1).any()
+    page = int(c.tab[0, 62])  # positions 992..: past the table
+    assert torch.equal(c.k[page], k0[page])
+    assert m27b.device_status() == 0
 
 
 def test_rope_append_out_of_range_is_left_out(torch, m27b):
