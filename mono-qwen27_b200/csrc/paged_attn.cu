@@ -275,8 +275,10 @@ struct PaSpan {
 // Units of an item: its key tiles, and the time between two items (the pipeline
 // drains, O leaves) in tiles.  Without it a worker with many short items runs
 // behind: a decode batch of 64 sequences of 300 to 8192 positions ended after
-// 103 us on the median CTA and 146 us on the last.
-constexpr int PA_EXTRA = 3, PAIR_EXTRA = 5;
+// 103 us on the median CTA and 146 us on the last.  Swept on that batch and
+// on a 4096-token chunk: 1, 2, 3, 4, 5, 6, 8 tiles 144, 133, 130, 122, 122, 123,
+// 126 us; pairs 4, 6, 8, 10, 12 tiles 430, 430, 434, 435, 468 us.
+constexpr int PA_EXTRA = 4, PAIR_EXTRA = 6;
 template <int EX>
 M27B_DI int pa_units(const PaSpan &s) { return s.kt1 - s.kt0 + EX; }
 template <int KT>

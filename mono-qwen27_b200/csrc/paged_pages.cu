@@ -88,15 +88,23 @@ M27B_DI int block_exclusive(int v, int *red, int *total) {
     return sat_add(warp ? red[warp - 1] : 0, inc - v);
 }
 
-// The lowest `want` free pages into fresh[]; false if there are fewer.
+// The lowest `want` free pages into fresh[]; false if there are fewer.  Four
+// pages a thread between two scans of the CTA.
 M27B_DI bool take_free(const int *ref, int n_pages, int want, int *fresh, int *red) {
     int got = 0;
-    for (int p0 = 0; p0 < n_pages && got < want; p0 += PLAN_THREADS) {
-        const int p = p0 + threadIdx.x;
-        const bool free = p < n_pages && ref[p] <= 0;
-        int total;
-        const int k = got + block_exclusive(free, red, &total);
-        if (free && k < want) fresh[k] = p;
+    for (int p0 = 0; p0 < n_pages && got < want; p0 += 4 * PLAN_THREADS) {
+        const int p = p0 + 4 * threadIdx.x;
+        bool free[4];
+        int n = 0, total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            free[i] = p + i < n_pages && ref[p + i] <= 0;
+            n += free[i];
+        }
+        int k = got + block_exclusive(n, red, &total);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (free[i] && k < want) fresh[k++] = p + i;
         got += total;
     }
     return got >= want;
@@ -213,6 +221,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_compact_plan(const PagesArgs a
         const int kh = holes + block_exclusive(hole, red, &nh), km = movers + block_exclusive(mover, red, &nm);
         if (hole) a.s.fresh[kh] = p;
         if (mover) a.s.from[km] = p;
+        else if (p < pg.n_pages) a.s.at[p] = -1;  // stays
         holes += nh;
         movers += nm;
     }
@@ -329,28 +338,22 @@ __global__ void __launch_bounds__(COPY_THREADS) k_compact_apply(const PagesArgs 
     pdl_wait();
     pdl_trigger();
     const M27BPages &pg = a.pg;
-    const int n = a.s.hdr->n_moves, live = a.s.hdr->n_live;
+    const int n = a.s.hdr->n_moves;
     if (n == 0) return;
     for (int r = blockIdx.x; r < pg.n_rows; r += gridDim.x) {
         const int h = min(held_pages(max(0, pg.lens[r]), pg.page_size), pg.n_cols);
         for (int c = threadIdx.x; c < h; c += COPY_THREADS) {
             int *e = pg.table + (size_t)r * pg.n_cols + c;
             const int p = *e;
-            if (p >= live && p < pg.n_pages && pg.ref[p] > 0) *e = a.s.at[p];
+            if (p >= 0 && p < pg.n_pages && a.s.at[p] >= 0) *e = a.s.at[p];
         }
     }
-    move_pages(a.pools, n, [&](int i) { return make_int2(a.s.from[i], a.s.fresh[i]); });
-}
-
-// The counts follow once no CTA reads the old ones.
-__global__ void __launch_bounds__(COPY_THREADS) k_compact_ref(const PagesArgs a) {
-    pdl_wait();
-    pdl_trigger();
-    const int n = a.s.hdr->n_moves;
+    // nothing here reads the counts: at[] says which pages move
     for (int k = blockIdx.x * COPY_THREADS + threadIdx.x; k < n; k += gridDim.x * COPY_THREADS) {
-        a.pg.ref[a.s.fresh[k]] = a.pg.ref[a.s.from[k]];
-        a.pg.ref[a.s.from[k]] = 0;
+        pg.ref[a.s.fresh[k]] = pg.ref[a.s.from[k]];
+        pg.ref[a.s.from[k]] = 0;
     }
+    move_pages(a.pools, n, [&](int i) { return make_int2(a.s.from[i], a.s.fresh[i]); });
 }
 
 __global__ void __launch_bounds__(COPY_THREADS) k_pages_free(const PagesArgs a) {
@@ -487,7 +490,6 @@ bool m27b_pages_compact(const M27BPages *pages, const M27BPagePool *pools, int n
     pages_scratch(pages->n_pages, pages->n_rows, 0, scratch, &a.s);
     cudaError_t e = launch_pdl(k_compact_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, a);
     if (e == cudaSuccess) e = launch_pdl(k_compact_apply, dim3(copy_grid()), dim3(COPY_THREADS), 0, stream, a);
-    if (e == cudaSuccess) e = launch_pdl(k_compact_ref, dim3(8), dim3(COPY_THREADS), 0, stream, a);
     return paged_ok(e, what, err, err_cap);
 }
 
