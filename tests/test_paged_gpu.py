@@ -707,3 +707,51 @@ def test_pages_graph(torch, m27b):
             u.ps.free(dst)
             u.ref.free([2, 3])
     u.same()
+
+
+# --------------------------------------------------------------------------
+# all of it together
+
+
+def test_example_runs(torch, m27b, capsys):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    ex.main()
+    assert "pages in use" in capsys.readouterr().out
+
+
+def test_forked_sequences_go_on_apart(torch, m27b):
+    # a fork, then different tokens: each row's cache is its own from there on,
+    # and equals one built without a fork
+    ps, n_kv, hd = 16, 2, 64
+    pool = torch.randn(2, 60, ps, n_kv, hd, device="cuda").bfloat16()
+    pages = m27b.PageSet.empty(4, 10, 60, ps, pool)
+    kv = m27b.PagedKV(pool[0], pool[1], pages.table)
+    rope, scr = m27b.rope_table(200, hd, 1e4), m27b.paged_attn_scratch(4, n_kv, hd)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def add(row, x):
+        n = len(x)
+        pages.resize(i(row), pages.lens[row:row + 1] + n)
+        q, o = (torch.empty(n, 4, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        m27b.rope_append(kv, x[:, :4], x[:, 4:6], x[:, 6:], i(0, n), pages.lens, rope, q, rows=i(row))
+        m27b.paged_attn(kv, q, i(0, n), pages.lens, o, scr, rows=i(row))
+        return o
+
+    x = [torch.randn(n, 8, hd, device="cuda") for n in (37, 5, 30, 1)]
+    add(0, x[0])
+    pages.fork(i(0), i(1))
+    left, right = add(0, x[1]), add(1, x[2])
+    right2 = add(1, x[3])
+    add(2, x[0])
+    assert torch.equal(add(2, x[1]), left)
+    pages.free(i(0, 2))
+    pages.compact()
+    add(3, x[0])
+    assert torch.equal(add(3, x[2]), right) and torch.equal(add(3, x[3]), right2)
+    pages.check()
+    assert int((pages.ref > 0).sum()) == 2 * P.cdiv(68, ps)
