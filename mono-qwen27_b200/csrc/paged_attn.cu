@@ -549,6 +549,17 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
     if (w.whole()) {
         if (idle) return;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const bool nothing = __any_sync(0xffffffffu, !(l > 0.0f));  // some row's O is not to be read
+        // where quadruple row & 3 of 32 columns of rows (row & ~3) .. + 3 goes
+        uint16_t *to[4];
+        int i = (row & ~3) / G, g = (row & ~3) - i * G;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            to[r] = (row & ~3) + r < rows ? (uint16_t *)a.out + (tok + i) * a.out_stride + (long long)(w.j * G + g) * HD + part * COLS +
+                                                8 * (row & 3)
+                                          : nullptr;
+            if (++g == G) g = 0, ++i;
+        }
 #pragma unroll 1
         for (int x = 0; x < COLS / 32; ++x) {
             uint32_t v[32];
@@ -556,6 +567,9 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
                 tmem_ld32(o + part * COLS + 32 * x, v);
                 tmem_wait_ld();
             }
+            if (nothing && !(l > 0.0f))
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = 0u;
             // four quadruples of 16 bits; then lane 4 g + j holds quadruple j of rows
             // 4 g .. 4 g + 3, so that a store has 64 bytes of a row together
             uint4 y[4];
@@ -564,19 +578,13 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
                 uint32_t z[4];
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
-                    z[d] = l > 0.0f ? Half16<BF>::down(__uint_as_float(v[8 * e + 2 * d]) * inv,
-                                                       __uint_as_float(v[8 * e + 2 * d + 1]) * inv)
-                                    : 0u;
+                    z[d] = Half16<BF>::down(__uint_as_float(v[8 * e + 2 * d]) * inv, __uint_as_float(v[8 * e + 2 * d + 1]) * inv);
                 y[e] = make_uint4(z[0], z[1], z[2], z[3]);
             }
             transpose4(y);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int other = (row & ~3) + r;
-                if (other < rows)
-                    *(uint4 *)((uint16_t *)a.out + (tok + other / G) * a.out_stride + (long long)(w.j * G + other % G) * HD +
-                               part * COLS + 32 * x + 8 * (row & 3)) = y[r];
-            }
+            for (int r = 0; r < 4; ++r)
+                if (to[r]) *(uint4 *)(to[r] + 32 * x) = y[r];
         }
         if (live && a.lse && part == 0)
             a.lse[at * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
@@ -930,9 +938,7 @@ static_assert(2 * PAIR_REGS_SOFTMAX + PAIR_REGS_OTHER <= 3 * 168, "register spli
 
 template <int HD> struct PairShared {
     PaRun run;
-    struct {
-        PaWalk<PairPlan<HD>::KT, PAIR_EXTRA> w;
-    } walk[PAIR_SOFTMAX];
+    PaWalk<PairPlan<HD>::KT, PAIR_EXTRA> walk[PAIR_SOFTMAX][2];  // of each softmax warp: the item at hand and the next
     PaItem tail[PAIR_SOFTMAX];
     AttnArgs args;
     long long red[PAIR_THREADS / 32];
@@ -1205,16 +1211,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             else pair_arrive(bar);
         };
         // the walk's state is in shared memory, for registers' sake
-        PaWalk<KT, PAIR_EXTRA> &w = sh.walk[warp].w;
-        if (lane == 0) w.begin(a, sh.run, tqw);
+        const int row_tok = row / G;
+        int cur = 0;
+        if (lane == 0) sh.walk[warp][0].begin(a, sh.run, tqw);
         __syncwarp();
-        while (ok && w.more()) {
+        while (ok && sh.walk[warp][cur].more()) {
+            const PaWalk<KT, PAIR_EXTRA> &w = sh.walk[warp][cur];
             const int n = w.tiles(), x_first = w.first() * KT;
             const int2 seen = pa_seen(w.s, a.window);
             const int i0 = w.r * tqw + rank * tq, rows = max(0, min(tq, w.s.q_n - i0)) * G;
             const bool live = row < rows, idle = 32 * quarter >= rows;  // idle: no row of this warp is live
             // a dead row's scores are garbage that no one reads
-            const int hi = live ? w.s.base + i0 + row / G + 1 : 0x7fffffff;
+            const int hi = live ? w.s.base + i0 + row_tok + 1 : 0x7fffffff;
             const int lo = live && a.window > 0 ? max(0, hi - a.window) : 0;
             float m = -INFINITY, l = 0.0f;  // m in units of c s; l of this warp's tiles
             for (int k = (wg ^ t0) & 1; k < n; k += 2) {
@@ -1318,6 +1326,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 if (lane == 0) arrive(&pfull[wg]);
             }
             if (!ok) break;
+            if (lane == 0) {
+                // the next item, while the last product runs
+                sh.walk[warp][cur ^ 1] = w;
+                sh.walk[warp][cur ^ 1].next(a);
+            }
             if (n > 0) {
                 const int last = t0 + n - 1;
                 if (!(ok = pa_warp_wait(&pdone[last & 1], (uint32_t)((last >> 1) & 1), abort, a.status))) break;
@@ -1345,8 +1358,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             }
             t0 += n;
             __syncwarp();
-            if (lane == 0) w.next(a);
-            __syncwarp();
+            cur ^= 1;
         }
         if (tid == 0) a.items[blockIdx.x] = sh.tail[0];
     }
