@@ -77,34 +77,17 @@ M27B_DI void load_head(const void *base, long long off, float (&x)[V]) {
     }
 }
 
-// The same from shared memory.
-template <bool F32, bool BF, int V>
-M27B_DI void load_head_smem(const uint8_t *base, int d0, float (&x)[V]) {
+// Eight values from shared memory.
+template <bool F32, bool BF>
+M27B_DI void load8_smem(const uint8_t *p, float (&x)[8]) {
     if constexpr (F32) {
-        const float *p = (const float *)base + d0;
-#pragma unroll
-        for (int c = 0; c < V / 2; ++c) {
-            if constexpr (V == 2) {
-                const float2 t = *(const float2 *)p;
-                x[0] = t.x, x[1] = t.y;
-            } else if (c % 2 == 0) {
-                const float4 t = *((const float4 *)p + c / 2);
-                x[2 * c] = t.x, x[2 * c + 1] = t.y, x[2 * c + 2] = t.z, x[2 * c + 3] = t.w;
-            }
-        }
+        const float4 u = *(const float4 *)p, v = *((const float4 *)p + 1);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
     } else {
-        uint32_t w[V / 2];
-        const uint16_t *p = (const uint16_t *)base + d0;
-        if constexpr (V == 2) w[0] = *(const uint32_t *)p;
-        else if constexpr (V == 4) {
-            const uint2 t = *(const uint2 *)p;
-            w[0] = t.x, w[1] = t.y;
-        } else {
-            const uint4 t = *(const uint4 *)p;
-            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
-        }
+        const uint4 u = *(const uint4 *)p;
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const float2 f = Half16<BF>::up(w[i]);
             x[2 * i] = f.x, x[2 * i + 1] = f.y;
         }
@@ -242,30 +225,72 @@ __global__ void __launch_bounds__(256) k_rope_append(const RopeArgs a) {
     else store_head<BF>(a.kv.k, k.slot + (long long)j * HD + d0, x);
 }
 
-// Many tokens: a unit is up to `per` heads of a token, at most 32 KB of
-// projections.  A producer warp looks the units' tokens up, 32 at a time, and
-// keeps ROPE_STAGES units in flight in shared memory (bulk copies of the unit's
-// q, k and v heads and of the position's row of the table); eight warps turn
-// them.  The lookups' and the memory's latency, which held the kernel above to
-// half of the bandwidth however its warps were sized (9.6k tokens of 32 heads
-// of 256 fp32 values: 85 us, floor 43), are then off the warps' path.
-constexpr int ROPE_STAGES = 3, ROPE_WARPS = 8;
-constexpr int ROPE_STAGE = 32 * 1024, ROPE_TAB = 1024;
-constexpr int ROPE_THREADS = (ROPE_WARPS + 1) * 32;
-constexpr size_t ROPE_SMEM = (size_t)ROPE_STAGES * (ROPE_STAGE + ROPE_TAB);
+// This lane's eight values of a head that LG lanes hold, normalised with
+// weights w (if `norm`) and turned (if `turn`).  For the half layout cs has the
+// sine's sign of the lane's place in the pair.  All lanes come here.
+template <int LG>
+M27B_DI void norm_turn8(const RopeArgs &a, bool norms, bool norm, bool turn, const float (&w)[8], const float2 (&cs)[8], int from, float (&x)[8]) {
+    if (norms) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+        for (int o = LG / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float sc = rsqrtf(fmaf(ss, 1.0f / (8 * LG), a.h.eps));
+        if (norm)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * sc * w[i];
+    }
+    if (a.rope.interleaved) {
+        if (turn)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = x[2 * i], v = x[2 * i + 1];
+                x[2 * i] = u * cs[i].x - v * cs[i].y, x[2 * i + 1] = u * cs[i].y + v * cs[i].x;
+            }
+    } else {
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], from);
+        if (turn)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i].x, o[i] * cs[i].y);
+    }
+}
 
-template <bool F32, bool BF, int V>
-__global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs a, int per, int groups, int wait_code) {
-    constexpr int HD = 32 * V, ES = F32 ? 4 : 2, HB = HD * ES;
+// Many tokens: a unit is up to p.per heads of a token, at most 32 KB of
+// projections.  A producer warp looks the units' tokens up, 32 at a time, and
+// keeps p.stages units in flight in shared memory (bulk copies of the unit's
+// q, k and v heads and of the position's row of the table); eight warps turn
+// them, a lane eight values of a head.  The lookups' and the memory's latency,
+// which hold the kernel above to half of the bandwidth, are then off the warps'
+// path.  8192 tokens, from cold L2: 32 heads of 256 fp32 values 135 -> 75 us
+// (403 MB, 5.4 TB/s), 32 heads of 128 bf16 values 102 -> 47 us (134 MB, 2.9
+// TB/s: there the warps' instructions bound it).  A warp with whole heads, as
+// above, took 80 and 57 us; 12 and 16 warps 80 and 98 us, 47 and 68 us.
+constexpr int ROPE_WARPS = 8, ROPE_MAX_STAGES = 8;
+constexpr int ROPE_UNIT = 32 * 1024;
+constexpr int ROPE_THREADS = (ROPE_WARPS + 1) * 32;
+constexpr int ROPE_SMEM = 110 * 1024;  // of a CTA, two on an SM
+
+// A unit's size and the stages that a CTA keeps of it.
+struct RopeStream {
+    int per, groups;         // heads of a unit, units of a token
+    int stage, tab, stages;  // bytes of a stage and of its row of the table
+};
+
+template <bool F32, bool BF, int LG>
+__global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs a, const RopeStream p, int wait_code) {
+    constexpr int HD = 8 * LG, ES = F32 ? 4 : 2, HB = HD * ES, HW = 32 / LG;  // HW: heads of a warp at once
     extern __shared__ __align__(128) uint8_t rope_smem[];
-    __shared__ uint64_t full[ROPE_STAGES], empty[ROPE_STAGES];
-    __shared__ long long slots[ROPE_STAGES];  // the unit's slot; -1: token left out
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d0 = lane * V;
+    __shared__ uint64_t full[ROPE_MAX_STAGES], empty[ROPE_MAX_STAGES];
+    __shared__ long long slots[ROPE_MAX_STAGES];  // the unit's slot; -1: token left out
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rows = a.h.n_q + 2 * a.kv.n_kv;
-    const long long units = (long long)a.bt.n_tok * groups, mine = blockIdx.x < units ? (units - 1 - blockIdx.x) / gridDim.x + 1 : 0;
-    uint8_t *tabs = rope_smem + (size_t)ROPE_STAGES * ROPE_STAGE;
+    const long long units = (long long)a.bt.n_tok * p.groups, mine = blockIdx.x < units ? (units - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+    uint8_t *tabs = rope_smem + (size_t)p.stages * p.stage;
     if (tid == 0) {
-        for (int s = 0; s < ROPE_STAGES; ++s) {
+        for (int s = 0; s < p.stages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], ROPE_WARPS);
         }
@@ -274,44 +299,52 @@ __global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs 
     __syncthreads();
     pdl_wait();
     pdl_trigger();
+    int s = 0;
+    uint32_t turn = 0;  // parity of the ring's round
+    // the unit at hand: group g of token t; gridDim.x units on
+    int t = (int)(blockIdx.x / p.groups), g = (int)(blockIdx.x % p.groups);
+    const int dt = (int)(gridDim.x / p.groups), dg = (int)(gridDim.x % p.groups);
+    auto step = [&] {
+        if (++s == p.stages) s = 0, turn ^= 1u;
+        t += dt, g += dg;
+        if (g >= p.groups) g -= p.groups, ++t;
+    };
     if (warp == ROPE_WARPS) {
         bool ok = true;
         RopeToken k = {-1, 0};
         long long n = 0;
         for (; ok && n < mine; ++n) {
-            const int s = (int)(n % ROPE_STAGES);
             if (n % 32 == 0) {
                 // the next 32 units' tokens, one a lane
                 const long long u = blockIdx.x + (n + lane) * (long long)gridDim.x;
                 k.slot = -1;
                 if (n + lane < mine) {
-                    const int t = (int)(u / groups);
+                    const int tl = (int)(u / p.groups);
                     int lo = 0, hi = a.bt.n_seq;
                     while (lo < hi) {
                         const int mid = (lo + hi) / 2;
-                        if (__ldg(a.bt.cu_q + mid + 1) <= t) lo = mid + 1;
+                        if (__ldg(a.bt.cu_q + mid + 1) <= tl) lo = mid + 1;
                         else hi = mid;
                     }
-                    if (!rope_token(a, t, lo, true, k)) k.slot = -1;
+                    if (!rope_token(a, tl, lo, true, k)) k.slot = -1;
                 }
                 __syncwarp();
             }
             const long long slot = __shfl_sync(0xffffffffu, k.slot, (int)(n % 32));
             const int rp = __shfl_sync(0xffffffffu, k.rp, (int)(n % 32));
             if (lane == 0) {
-                if (n >= ROPE_STAGES && !mbar_wait_bounded(&empty[s], (uint32_t)((n / ROPE_STAGES - 1) & 1), a.status, wait_code)) ok = false;
+                if (n >= p.stages && !mbar_wait_bounded(&empty[s], turn ^ 1u, a.status, wait_code)) ok = false;
                 else {
-                    const long long u = blockIdx.x + n * (long long)gridDim.x;
-                    const int t = (int)(u / groups), r0 = (int)(u - (long long)t * groups) * per, r1 = min(rows, r0 + per);
+                    const int r0 = g * p.per, r1 = min(rows, r0 + p.per);
                     slots[s] = slot;
                     if (slot < 0) mbar_arrive_local(&full[s]);
                     else {
                         const int nq = max(0, min(r1, a.h.n_q) - r0), kb = a.h.n_q + a.kv.n_kv;
                         const int k0 = max(r0, a.h.n_q), nk = max(0, min(r1, kb) - k0), v0 = max(r0, kb), nv = max(0, r1 - v0);
-                        uint8_t *st = rope_smem + (size_t)s * ROPE_STAGE;
+                        uint8_t *st = rope_smem + (size_t)s * p.stage;
                         const uint32_t tb = (uint32_t)a.rope.n_rot * 4;
                         mbar_arrive_expect_tx(&full[s], (uint32_t)(r1 - r0) * HB + tb);
-                        bulk_copy_g2s(tabs + s * ROPE_TAB, a.rope.table + (long long)rp * a.rope.n_rot, tb, &full[s]);
+                        bulk_copy_g2s(tabs + s * p.tab, a.rope.table + (long long)rp * a.rope.n_rot, tb, &full[s]);
                         if (nq) bulk_copy_g2s(st, (const uint8_t *)a.h.q + (t * a.h.q_stride + (long long)r0 * HD) * ES, nq * HB, &full[s]);
                         if (nk)
                             bulk_copy_g2s(st + (k0 - r0) * HB, (const uint8_t *)a.h.k + (t * a.h.k_stride + (long long)(k0 - a.h.n_q) * HD) * ES,
@@ -323,59 +356,77 @@ __global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs 
                 }
             }
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            step();
         }
         // every copy lands before the shared memory is released (bounded)
         if (lane == 0)
-            for (long long i = ok ? n : n - 1, e = i; i > 0 && e - i < ROPE_STAGES; --i)
-                mbar_wait_bounded(&full[(i - 1) % ROPE_STAGES], (uint32_t)(((i - 1) / ROPE_STAGES) & 1), a.status, wait_code);
+            for (long long i = ok ? n : n - 1, e = i; i > 0 && e - i < p.stages; --i) {
+                const long long round = (i - 1) / p.stages;
+                mbar_wait_bounded(&full[(i - 1) - round * p.stages], (uint32_t)(round & 1), a.status, wait_code);
+            }
         return;
     }
-    float qw[V], kw[V];
-    if (a.h.q_norm) norm_weights<V>(a.h.q_norm, d0, qw);
-    if (a.h.k_norm) norm_weights<V>(a.h.k_norm, d0, kw);
+    const int d0 = 8 * (lane % LG), half = a.rope.n_rot / 2, kb = a.h.n_q + a.kv.n_kv;
+    const bool turns = d0 < a.rope.n_rot, first = d0 < half, norms = a.h.q_norm || a.h.k_norm;
+    const int from = first ? lane + half / 8 : lane - half / 8;  // the lane with the pairs' other values
+    float qw[8] = {}, kw[8] = {};
+    if (a.h.q_norm) norm_weights<8>(a.h.q_norm, d0, qw);
+    if (a.h.k_norm) norm_weights<8>(a.h.k_norm, d0, kw);
     for (long long n = 0; n < mine; ++n) {
-        const int s = (int)(n % ROPE_STAGES);
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (uint32_t)((n / ROPE_STAGES) & 1), a.status, wait_code))) return;
-        const long long u = blockIdx.x + n * (long long)gridDim.x, slot = slots[s];
-        const int t = (int)(u / groups), r0 = (int)(u - (long long)t * groups) * per, r1 = min(rows, r0 + per);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], turn, a.status, wait_code))) return;
+        const long long slot = slots[s];
+        const int r0 = g * p.per, r1 = min(rows, r0 + p.per);
         if (slot >= 0) {
-            float2 cs[V];
-            rope_factors<V>(a, (const float2 *)(tabs + s * ROPE_TAB), d0, cs);
-            for (int r = r0 + warp; r < r1; r += ROPE_WARPS) {
-                float x[V];
-                load_head_smem<F32, BF>(rope_smem + (size_t)s * ROPE_STAGE + (r - r0) * HB, d0, x);
-                const int j = r - a.h.n_q;
-                if (r < a.h.n_q) {
-                    norm_turn<V>(a, a.h.q_norm != nullptr, qw, cs, d0, lane, x);
-                    store_head<BF>(a.q_out, t * a.q_out_stride + (long long)r * HD + d0, x);
-                } else if (j < a.kv.n_kv) {
-                    norm_turn<V>(a, a.h.k_norm != nullptr, kw, cs, d0, lane, x);
-                    store_head<BF>(a.kv.k, slot + (long long)j * HD + d0, x);
-                } else store_head<BF>(a.kv.v, slot + (long long)(j - a.kv.n_kv) * HD + d0, x);
+            uint16_t *qo = (uint16_t *)a.q_out + t * a.q_out_stride + d0;
+            uint16_t *ko = (uint16_t *)a.kv.k + slot + d0, *vo = (uint16_t *)a.kv.v + slot + d0;
+            const uint8_t *st = rope_smem + (size_t)s * p.stage;
+            float2 cs[8];
+            rope_factors<8>(a, (const float2 *)(tabs + s * p.tab), d0, cs);
+            if (!a.rope.interleaved && first)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) cs[i].y = -cs[i].y;
+            for (int rw = r0 + warp * HW; rw < r1; rw += HW * ROPE_WARPS) {
+                const int r = min(rw + lane / LG, r1 - 1);
+                float x[8];
+                load8_smem<F32, BF>(st + (r - r0) * HB + d0 * ES, x);
+                const bool is_q = r < a.h.n_q, is_v = r >= kb;
+                if (rw < kb) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = is_q ? qw[i] : kw[i];
+                    norm_turn8<LG>(a, norms, is_q ? a.h.q_norm != nullptr : !is_v && a.h.k_norm, turns && !is_v, w, cs, from, x);
+                }
+                if (rw + lane / LG < r1) store_head<BF>(is_q ? qo : is_v ? vo : ko, (is_q ? r : is_v ? r - kb : r - a.h.n_q) * HD, x);
             }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_local(&empty[s]);
+        step();
     }
 }
 
 template <bool F32, bool BF, int V>
 cudaError_t rope_launch_v(const RopeArgs &a, cudaStream_t st) {
     const int rows = a.h.n_q + 2 * a.kv.n_kv, hb = 32 * V * (F32 ? 4 : 2);
-    const int per = ROPE_STAGE / hb < rows ? ROPE_STAGE / hb : rows, groups = (rows + per - 1) / per;
-    const long long units = (long long)a.bt.n_tok * groups, ctas = 2 * 148;
-    // the stream once every CTA's stages fill twice over
-    if (units >= ctas * 2 * ROPE_STAGES) {
+    RopeStream p;
+    p.per = ROPE_UNIT / hb < rows ? ROPE_UNIT / hb : rows, p.groups = (rows + p.per - 1) / p.per;
+    const long long units = (long long)a.bt.n_tok * p.groups, ctas = 2 * 148;
+    // the stream once a CTA has two units (32 heads, microseconds by head and by
+    // stream from cold L2: fp32 of 256, 148 tokens 10.2 and 12.3, 592 16.4 and
+    // 16.4, 1184 26.6 and 20.5; bf16 of 128, 8.2 and 10.2, 14.3 and 12.3, 20.5 and 14.5)
+    if (units >= ctas * 2) {
+        p.stage = p.per * hb, p.tab = (a.rope.n_rot * 4 + 127) & ~127;
+        p.stages = ROPE_SMEM / (p.stage + p.tab) < ROPE_MAX_STAGES ? ROPE_SMEM / (p.stage + p.tab) : ROPE_MAX_STAGES;
         static bool ready[64] = {};
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         if (dev < 0 || dev >= 64 || !ready[dev]) {
-            e = cudaFuncSetAttribute(k_rope_stream<F32, BF, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ROPE_SMEM);
+            e = cudaFuncSetAttribute(k_rope_stream<F32, BF, 4 * V>, cudaFuncAttributeMaxDynamicSharedMemorySize, ROPE_SMEM);
             if (e != cudaSuccess) return e;
             if (dev >= 0 && dev < 64) ready[dev] = true;
         }
-        return launch_pdl(k_rope_stream<F32, BF, V>, dim3((unsigned)ctas), dim3(ROPE_THREADS), ROPE_SMEM, st, a, per, groups, 5);
+        return launch_pdl(k_rope_stream<F32, BF, 4 * V>, dim3((unsigned)ctas), dim3(ROPE_THREADS), (size_t)p.stages * (p.stage + p.tab), st, a, p, 5);
     }
     const dim3 grid((unsigned)(((long long)a.bt.n_tok * rows + 7) / 8)), block(256);
     return launch_pdl(k_rope_append<F32, BF, V>, grid, block, 0, st, a);

@@ -420,13 +420,15 @@ def test_attn_bad_pages_are_reported(torch, m27b):
 
 
 def _check_rope(torch, m27b, q_lens, kv_lens, n_q, n_kv, hd, dtype, src, ps, n_rot, interleaved, norm, seed, pad=0,
-                rows=None, positions=None, in_place=False):
+                rows=None, positions=None, in_place=False, v_inf=False):
     c = Cache(torch, m27b, kv_lens, ps, n_kv, hd, dtype, seed, pad=pad, rows=rows, poison=False)
     before = _np(c.k), _np(c.v)
     g = torch.Generator(device="cuda").manual_seed(seed + 1)
     total, heads = sum(q_lens), n_q + 2 * n_kv
     x = (3 * torch.randn(total, heads, hd, generator=g, device="cuda")).to(_dt(torch, src))
-    w = [1 + 0.3 * torch.randn(hd, generator=g, device="cuda") for _ in range(2)] if norm else [None, None]
+    w = [1 + 0.3 * torch.randn(hd, generator=g, device="cuda") if norm in (True, s) else None for s in "qk"]
+    if v_inf:
+        x[::7, n_q + n_kv:, ::5] = float("inf")
     xn = _np(x)
     z = P.rope_factors(max(kv_lens) + 50, n_rot, 1e4)
     tab = torch.from_numpy(np.stack([z.real, z.imag], -1).astype(np.float32)).cuda().contiguous()
@@ -503,6 +505,14 @@ def test_rope_append_many_tokens(torch, m27b, n_q, n_kv, hd, src, dtype, ps, int
     # enough tokens for the streaming kernel; 40 + 16 heads of 256 fp32 values are two units a token
     _check_rope(torch, m27b, [1200, 0, 700], [1200, 5, 1000], n_q, n_kv, hd, dtype, src, ps, hd // 2, interleaved, True, seed=50,
                 rows=[2, 0, 1])
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd,n_rot,norm", [(3, 2, 64, 16, "q"), (5, 1, 64, 48, "k"), (5, 3, 128, 32, "k"),
+                                                    (1, 1, 128, 16, True), (3, 2, 256, 16, "q"), (9, 5, 128, 128, True)])
+def test_rope_append_many_tokens_mixed_heads(torch, m27b, n_q, n_kv, hd, n_rot, norm):
+    # q, k and v heads in one warp, of which only some are normalised and turned
+    _check_rope(torch, m27b, [640, 1, 9], [700, 1, 30], n_q, n_kv, hd, "bf16", "f32", 16, n_rot, False, norm, seed=53, v_inf=True)
+    _check_rope(torch, m27b, [650], [651], n_q, n_kv, hd, "f16", "f16", 64, n_rot, True, norm, seed=54, v_inf=True)
 
 
 def test_rope_append_many_tokens_in_place_and_left_out(torch, m27b):
