@@ -19,31 +19,40 @@
 // per worker in the scratch, and a second launch, whose blocks wait on the
 // SMs for the first to end, adds the records in worker order.
 //
-// A worker is one CTA (one per SM), or with PAIR a cluster of two CTAs that
-// take 128 rows each and share the key tiles: each loads half of K's positions
-// and half of V's columns, and the MMAs of the pair (cta_group::2, M = 256) read
-// both halves.  A single CTA's 128 rows need 64 KB of keys and values per
-// 1024 cycles of tensor work (head_dim 256, 64 positions), which the shared
-// memory cannot take in and hand to the MMAs at that rate; a pair needs half.
+// A worker is one CTA (k_paged_attn, one per SM), or for many rows a cluster of
+// two CTAs (k_paged_attn_pair) that take 128 rows each and share the key tiles:
+// each loads half of K's positions and half of V's columns, and the MMAs of the
+// pair (cta_group::2, M = 256) read both halves.  A single CTA's 128 rows need
+// 64 KB of keys and values per 1024 cycles of tensor work (head_dim 256, 64
+// positions), which the shared memory cannot take in and hand to the MMAs at
+// that rate; a pair needs half.
 //
-// A CTA's roles (12 warps):
+// What bounds it: decode (64 sequences of 300 to 8192 positions, 24 heads of
+// 256 over 4, 680 MB of cache) the memory: 120 us, 5.7 TB/s; a chunk of 4096
+// tokens over 8192 positions, same heads, the tensor pipe: 387 us with the pipe
+// busy 83 % of it at full clocks, 420 to 460 us (1.35 PFLOP/s) under the power
+// limit; few rows and short contexts the latency of the launch, the first loads
+// and the join: 13 us for one token over 769 positions.
+//
+// A CTA's roles:
 //   * warp 8 streams the key tiles into a ring of slots, in the order in which
 //     the MMAs use them (K0 K1 V0 K2 V1 ...): TMA boxes of 64 values x the
 //     positions of a page (or of the tile, if a page is longer), 128-byte
 //     swizzle, each lane one box; a page outside the item's positions is a box
 //     past the end of the pool, which reads zeros;
 //   * warp 9 issues the MMAs: S = Q K^T with K (K-major) in shared memory, O += P
-//     V with P in TMEM and V (N-major) in shared memory.  Q is in TMEM, or with
-//     PAIR in shared memory.  In a pair the first CTA's warp issues;
-//   * warps 0-7 have half a row per thread, warps w and w + 4 the halves of the
-//     same rows: the softmax of S (the two halves tell each other their
-//     maximum), P into TMEM, and at the item's end O / l to global memory.  A
-//     warp none of whose rows is live (decode: G rows of 128) only passes the
-//     barriers.
-// TMEM (512 columns): O | Q | S | P, P (PAIR: O | S | P, P).  S is free again
-// once the warps have loaded it, so the next product runs while they compute;
-// P has two buffers.  Steady state of the tensor pipe: P V of tile t, Q K of
-// tile t + 2, P V of tile t + 1, ...
+//     V with P in TMEM and V (N-major) in shared memory.  Q is in TMEM, in a
+//     pair in shared memory.  In a pair the first CTA's warp issues;
+//   * warps 0-7: the softmax of S, P into TMEM, and at the item's end O / l to
+//     global memory.  In a single CTA warps w and w + 4 have the halves of the
+//     same rows and tell each other their maximum (one tile's latency counts:
+//     decode has few live rows); in a pair they take turns with whole tiles
+//     and hand m on (throughput counts).  A warp none of whose rows is live
+//     (decode: G rows of 128) only passes the barriers.
+// TMEM (512 columns): O | Q | S | P, P (a pair: O | S (, S) | P, P).  S is free
+// again once the warps have loaded it, so the next product runs while they
+// compute; P has two buffers.  Steady state of the tensor pipe: P V of tile t,
+// Q K of tile t + 2, P V of tile t + 1, ...
 //
 // m moves only when the running maximum has grown by more than 2^8 since it
 // was set: weights then stay below 2^8 (fp32 sums, and far from the 16-bit
@@ -1604,8 +1613,14 @@ bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const v
     if (ctas < 2) return paged_fail(err, err_cap, "%s: no CUDA device", what);
     const AttnArgs a = {*kv, *batch, q, out, lse, q_stride, out_stride, n_q, window > 0 ? window : 0, scale,
                         (PaItem *)scratch, (float *)((char *)scratch + PA_MAX_CTAS * sizeof(PaItem)), status_ptr_current()};
-    // pairs of CTAs when a sequence has rows for both, on average
-    const bool pair = (long long)batch->n_tok * G >= 256ll * batch->n_seq;
+    // Pairs of CTAs when a sequence has rows for one and a half, on average.  With
+    // 128, 192, 256, 512 rows a sequence, microseconds by single CTAs and by pairs
+    // from cold L2: 16 sequences of 2000 positions, head_dim 256: 62 72 78 140 and
+    // 64 68 72 132; head_dim 128: 62 83 87 134 and 70 72 74 111; one sequence: 42 36
+    // 38 36 and 36 38 40 38; a prompt of 4096 tokens over 8192 positions, 24 heads of
+    // 256: 695 and 458, 16 heads of 128: 269 and 218.  (head_dim 64 has no pairs:
+    // a slot of 128 positions is 16 KB, and the shared memory keeps up.)
+    const bool pair = (long long)batch->n_tok * G >= 192ll * batch->n_seq;
     bool maps = false;
     const cudaError_t e = kv->type == M27B_TYPE_BF16 ? pa_launch_hd<true>(a, G, pair, ctas, stream, &maps)
                                                      : pa_launch_hd<false>(a, G, pair, ctas, stream, &maps);
