@@ -1381,6 +1381,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     }
 }
 
+constexpr int JOIN_THREADS = 128;
+
 // Add up the records of item blockIdx.x (the tail of that CTA's run, if it has
 // one) and write its rows.  A group of SP threads takes eight values of a row;
 // thread p has parts p, p + SP, ..., four in flight, and the group adds its
@@ -1390,7 +1392,7 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
     const int G = a.n_q / a.kv.n_kv, p = threadIdx.x % SP;
     const int first = blockIdx.x;
     auto record = [&](int x) { return a.part + (size_t)(2 * (first + stride * x) + (x == 0 ? 1 : 0)) * pa_record(HD); };
-    const int n = it.rows * (HD / 8), per = 256 / SP;
+    const int n = it.rows * (HD / 8), per = JOIN_THREADS / SP;
     for (int e0 = blockIdx.y * per; e0 < n; e0 += gridDim.y * per) {
         const int e = min(n - 1, e0 + (int)threadIdx.x / SP), d8 = e / it.rows, row = e - d8 * it.rows;
         float m = -INFINITY, l = 0.0f, o[8] = {};
@@ -1451,15 +1453,20 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
     }
 }
 
+// 80 registers of 128 threads fit on an SM beside a CTA of k_paged_attn, so that
+// the first blocks wait there for its end (verify 29.5 -> 28.6 us, one token over
+// 131071 positions 95.4 -> 93.8 us against blocks of 256).  Blocks that share
+// the tasks of all items evenly took 1 to 5 us more: the scan of the items comes
+// before the first read of a record.
 template <int HD, bool BF>
-__global__ void __launch_bounds__(256, 4) k_paged_join(const AttnArgs a, int stride) {
+__global__ void __launch_bounds__(JOIN_THREADS, 6) k_paged_join(const AttnArgs a, int stride) {
     pdl_wait();
     pdl_trigger();
     const PaItem it = a.items[blockIdx.x];
     if (it.np == 0) return;
     // the group size with the fewest round trips: those of a value (four parts
     // a thread each), times the values of a group
-    const int tasks = it.rows * (HD / 8), threads = 256 * gridDim.y;
+    const int tasks = it.rows * (HD / 8), threads = JOIN_THREADS * gridDim.y;
     auto trips = [&](int sp) { return (tasks * sp + threads - 1) / threads * (2 * ((it.np + 4 * sp - 1) / (4 * sp)) + 1); };
     const int t1 = trips(1), t2 = trips(2), t8 = trips(8);
     if (t1 <= t2 && t1 <= t8) pa_join<HD, BF, 1>(a, it, stride);
@@ -1544,7 +1551,7 @@ cudaError_t pa_join_launch(const AttnArgs &a, int ctas, int stride, cudaStream_t
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    return launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 8), dim3(256), 0, st, a, stride);
+    return launch_pdl(k_paged_join<HD, BF>, dim3(ctas, 16), dim3(JOIN_THREADS), 0, st, a, stride);
 }
 
 template <int HD, bool BF>
