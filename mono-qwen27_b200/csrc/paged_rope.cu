@@ -264,8 +264,8 @@ M27B_DI void norm_turn8(const RopeArgs &a, bool norms, bool norm, bool turn, con
 // q, k and v heads and of the position's row of the table); eight warps turn
 // them, a lane eight values of a head.  The lookups' and the memory's latency,
 // which hold the kernel above to half of the bandwidth, are then off the warps'
-// path.  8192 tokens, from cold L2: 32 heads of 256 fp32 values 135 -> 75 us
-// (403 MB, 5.4 TB/s), 32 heads of 128 bf16 values 102 -> 47 us (134 MB, 2.9
+// path.  8192 tokens, from cold L2: 32 heads of 256 fp32 values 135 -> 74 us
+// (403 MB, 5.4 TB/s), 32 heads of 128 bf16 values 102 -> 43 us (134 MB, 3.1
 // TB/s: there the warps' instructions bound it).  A warp with whole heads, as
 // above, took 80 and 57 us; 12 and 16 warps 80 and 98 us, 47 and 68 us.
 constexpr int ROPE_WARPS = 8, ROPE_MAX_STAGES = 8;
@@ -385,7 +385,9 @@ __global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs 
             if (!a.rope.interleaved && first)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) cs[i].y = -cs[i].y;
-            for (int rw = r0 + warp * HW; rw < r1; rw += HW * ROPE_WARPS) {
+            // the warps take turns at the unit's rows, since the v heads are little
+            // work (8192 tokens of 32 bf16 heads of 128: 45 -> 43 us)
+            for (int rw = r0 + (warp + 3 * (int)n) % ROPE_WARPS * HW; rw < r1; rw += HW * ROPE_WARPS) {
                 const int r = min(rw + lane / LG, r1 - 1);
                 float x[8];
                 load8_smem<F32, BF>(st + (r - r0) * HB + d0 * ES, x);
