@@ -1025,11 +1025,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     uint8_t *ring = smem + L::Q_BYTES;
     uint64_t *bars = (uint64_t *)(ring + (size_t)NS * SLOT);
     // full: a slot's copies have landed (in the first CTA, for those of both);
-    // empty: its MMAs are done; sfull, pdone, empty, qempty come to both CTAs;
-    // sfree, pfull, oread are the first CTA's, for the warps of both; vlanded tells
-    // the second CTA's softmax warps that a tile's V is there
+    // empty: its MMAs are done; sfull, pdone, odone, empty, qempty come to both
+    // CTAs; sfree, pfull, oread are the first CTA's, for the warps of both; vlanded
+    // tells the second CTA's softmax warps that a tile's V is there; odone has a
+    // phase an item
     uint64_t *full = bars, *empty = full + NS, *qfull = empty + NS, *qempty = qfull + 1, *vlanded = qempty + 1, *sfull = vlanded + 2, *sfree = sfull + 2, *pfull = sfree + 2, *pdone = pfull + 2,
-             *oread = pdone + 2, *drain = oread + 1, *pair = drain + 1;
+             *oread = pdone + 2, *odone = oread + 1, *drain = odone + 1, *pair = drain + 1;
     __shared__ PairShared<HD> sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x & 1, me = blockIdx.x >> 1;
@@ -1050,6 +1051,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             mbar_init(qfull, 1);
             mbar_init(qempty, 1);
             mbar_init(oread, 2 * PAIR_SOFTMAX);
+            mbar_init(odone, 1);
             mbar_init(drain, 1);
             sh.abort = 0;
         }
@@ -1188,6 +1190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     used();
                     pair_commit(lead, pdone0 + 8 * (v & 1));
                 }
+                if (ok) pair_commit(lead, smem_u32(odone));
                 ++item;
             }
             // every MMA issued above (bounded, even after an abort)
@@ -1205,6 +1208,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
         const float c = a.scale * 1.44269504088896340736f;  // log2 e
         int t0 = 0, u0 = 0, told = 0, zeroed = 0;  // u0: tiles of this quarter so far (of items where it has live rows)
+        uint32_t ended = 0;                        // parity of odone's phase
         bool ok = true;
         if (lane == 0) sh.tail[warp] = PaItem{0, 0, 0, 0};
         // m after tile u of this quarter, from the warp that has the tile to the
@@ -1341,10 +1345,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 sh.walk[warp][cur ^ 1].next(a);
             }
             if (n > 0) {
-                const int last = t0 + n - 1;
-                if (!(ok = pa_warp_wait(&pdone[last & 1], (uint32_t)((last >> 1) & 1), abort, a.status))) break;
+                // The item's products.  Not pdone of the last tile: the group that
+                // does not own it may know pdone of four tiles ago only, and the
+                // parity of a phase two early passes at once; an idle warp would
+                // then arrive on oread while the item before is still being read.
+                if (!(ok = pa_warp_wait(odone, ended, abort, a.status))) break;
+                ended ^= 1u;
                 tc_fence_after();
                 if (!idle) {
+                    const int last = t0 + n - 1;
                     // m of the last tile, and the other warp's sum under it
                     float end = m, theirs;
                     if ((last & 1) != wg && !(ok = follow(u0 + n - 1, end))) break;

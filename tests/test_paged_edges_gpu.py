@@ -1,0 +1,89 @@
+"""Edges of the paged attention on the GPU (include/m27b_paged.h) against a
+plain 64-bit computation.
+
+Tolerances: those of tests/test_paged_gpu.py (u: half a unit in the last place,
+relative; ds: the scores' fp32 sums).  A weight below f16's 2^-14 has an error of
+at most 2^-25 absolute; the largest weight is at least 2^7, so that adds at most
+2^-32 sum |v| for f16."""
+import random
+
+import numpy as np
+import pytest
+
+import _paged_ref as P
+from test_paged_gpu import Cache, _cu
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(torch, q, k, v, scale, window):
+    """One sequence: out, lse, sum p |v|, the row's largest scale * sum |q| |k|, and sum |v|."""
+    nq, n_q, hd = q.shape
+    nkv, n_kv = k.shape[:2]
+    q, k, v = q.double(), k.double().repeat_interleave(n_q // n_kv, 1), v.double().repeat_interleave(n_q // n_kv, 1)
+    hi = torch.arange(nq, device="cuda") + nkv - nq + 1
+    pos = torch.arange(nkv, device="cuda")
+    see = pos < hi[:, None]
+    if window > 0:
+        see &= pos >= hi[:, None] - window
+    see = see[:, None]
+    s = (scale * torch.einsum("thd,xhd->thx", q, k)).masked_fill(~see, -np.inf)
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - lse.masked_fill(lse == -np.inf, 0.0)[..., None])
+    big = (scale * torch.einsum("thd,xhd->thx", q.abs(), k.abs())).masked_fill(~see, 0.0)
+    big = big.amax(-1) if nkv else lse.masked_fill(lse == -np.inf, 0.0)
+    some = torch.einsum("thx,xhd->thd", see.expand_as(s).double(), v.abs())
+    return torch.einsum("thx,xhd->thd", p, v), lse, torch.einsum("thx,xhd->thd", p, v.abs()), big, some
+
+
+def _close(torch, got, lse, want, dtype):
+    out, l, mag, big, some = want
+    ds, u = 2.0 ** -19 * big + 1e-6, P.U[dtype]
+    tol = u * out.abs() + (u + 2 * ds[..., None]) * mag * 1.02 + 1e-7
+    if dtype == "f16":
+        tol = tol + 2.0 ** -32 * some
+    err = (got.double() - out).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+    if lse is not None:
+        f = torch.isfinite(l)
+        assert torch.equal(lse == -np.inf, l == -np.inf)
+        assert bool(((lse.double() - l).abs() <= ds + 1e-6 * (1 + l.abs()))[f].all())
+
+
+def _seq(torch, c, b):
+    n = c.lens_list[b]
+    ids = c.table[c.rows[b], :P.cdiv(n, c.ps)].long()
+    return tuple(x[ids].reshape(-1, *x.shape[2:])[:n] for x in (c.k, c.v))
+
+
+def _run(torch, m27b, c, q, cu, **kw):
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    m27b.paged_attn(c.kv, q, cu, c.lens, out, m27b.paged_attn_scratch(q.shape[1], c.kv.n_kv, q.shape[2]), lse=lse,
+                    rows=c.rows_t, **kw)
+    return out, lse
+
+
+@pytest.mark.parametrize("hd,dtype,n_q,n_kv", [(128, "f16", 16, 8), (128, "bf16", 12, 2), (256, "bf16", 12, 2)])
+def test_items_of_one_two_and_three_tiles_with_idle_quarters(torch, m27b, hd, dtype, n_q, n_kv):
+    # many prompts whose row tiles see one key tile, two and three, the last ones
+    # with idle warps or an idle second CTA, so that a pair has such items in a row
+    rng = random.Random(50)
+    per = 2 * (128 // (n_q // n_kv))  # tokens of a pair's item
+    q_lens = [rng.choice([per, 2 * per + 1, 2 * per + per // 3, 3 * per, per + 5, 3 * per + 1]) for _ in range(70)]
+    if per < 128:  # key tiles of 128 positions
+        kv = [n + rng.choice([0, 0, 128 - per, 256 - per, 300]) for n in q_lens]
+    else:
+        kv = list(q_lens)
+    c = Cache(torch, m27b, kv, 16, n_kv, hd, dtype, 51)
+    q = torch.randn(sum(q_lens), n_q, hd, device="cuda").to(c.k.dtype)
+    cu = _cu(torch, q_lens)
+    out, lse = _run(torch, m27b, c, q, cu)
+    at = 0
+    for b, n in enumerate(q_lens):
+        if b % 7 == 0:
+            _close(torch, out[at:at + n], lse[at:at + n], _attend(torch, q[at:at + n], *_seq(torch, c, b), hd ** -0.5, 0), dtype)
+        at += n
+    for _ in range(200):
+        again, lse2 = _run(torch, m27b, c, q, cu)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+    assert m27b.device_status() == 0

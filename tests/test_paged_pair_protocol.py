@@ -1,0 +1,222 @@
+"""The hand-offs of k_paged_attn_pair (mono-qwen27_b200/csrc/paged_attn.cu) as
+a model on the CPU: the roles of both CTAs as coroutines over barriers that know
+only a phase's parity, as the hardware's do, run in many random orders.
+
+An mbarrier wait names a parity, so one that comes two phases early passes at
+once.  The model counts phases, and calls a fault: a wait that passes for
+another phase than it means, an arrival in another phase than it means, a
+product that overwrites O before every live warp has read it, and a standstill."""
+import random
+
+import pytest
+
+AHEAD = 2  # products Q K ahead of P V
+
+
+class Fault(Exception):
+    pass
+
+
+class Bar:
+    def __init__(self, count):
+        self.count = self.left = count
+        self.done = 0  # phases completed
+
+    def arrive(self, phase=None):
+        if phase is not None and phase != self.done:
+            raise Fault("arrival in another phase")
+        self.left -= 1
+        if self.left == 0:
+            self.left, self.done = self.count, self.done + 1
+
+
+def wait(bar, phase):
+    """Until the parity says that `phase` is complete."""
+    while (bar.done & 1) == (phase & 1):
+        yield lambda: (bar.done & 1) != (phase & 1)
+    if bar.done != phase + 1:
+        raise Fault("wait passed for another phase")
+
+
+class Pair:
+    """One worker's run.  items: (tiles, live quarters of CTA 0, of CTA 1, first
+    and last tile with unseen positions).  end: what the end of an item waits
+    for, "item" (a barrier with a phase an item) or "tile" (the last tile's)."""
+
+    def __init__(self, items, slots, buffers, rng, quarters=2, end="item"):
+        self.items, self.ns, self.nb, self.rng, self.nq, self.end = items, slots, buffers, rng, quarters, end
+        n = 2 * quarters
+        two = lambda c: [Bar(c), Bar(c)]  # noqa: E731
+        # the first CTA's barriers, except where a list over the CTAs is named
+        self.full = [Bar(3) for _ in range(slots)]  # the expected bytes, and both CTAs' copies
+        self.empty = [[Bar(1) for _ in range(slots)] for _ in range(2)]
+        self.qfull, self.qempty = Bar(3), two(1)
+        self.sfull, self.pdone = [two(1), two(1)], [two(1), two(1)]
+        self.sfree, self.pfull, self.oread = two(n), two(n), Bar(2 * n)
+        self.odone, self.vlanded = two(1), two(1)
+        self.meet = [[Bar(2) for _ in range(quarters)] for _ in range(2)]
+        self.m = {}        # (CTA, quarter, tile's parity) -> tile, the running maximum's mailbox
+        self.pipe = []     # MMAs and commits, in order
+        self.reading = {}  # O of item i: live warps that have yet to read it
+        self.over = False
+
+    def producer(self, rank):
+        g = 0
+        for item, (n, *_) in enumerate(self.items):
+            for i in range(n + AHEAD):
+                for what in ("k", "q", "v"):
+                    if (what == "k" and i >= n) or (what == "q" and i > 0) or (what == "v" and i < AHEAD):
+                        continue
+                    if what == "q":
+                        if item:
+                            yield from wait(self.qempty[rank], item - 1)
+                        bar = self.qfull
+                    else:
+                        if g >= self.ns:
+                            yield from wait(self.empty[rank][g % self.ns], g // self.ns - 1)
+                        bar, g = self.full[g % self.ns], g + 1
+                    if rank == 0:
+                        bar.arrive()
+                    yield None
+                    bar.arrive()  # the copy lands
+
+    def issuer(self):
+        t = g = 0
+        for item, (n, *_) in enumerate(self.items):
+            yield from wait(self.qfull, item)
+            for i in range(n + AHEAD):
+                if i < n:
+                    if t >= self.nb:
+                        yield from wait(self.sfree[(t - self.nb) & 1], (t - self.nb) >> 1)
+                    yield from wait(self.full[g % self.ns], g // self.ns)
+                    self.pipe += [("commit", [self.sfull[r][t & 1] for r in (0, 1)]),
+                                  ("commit", [self.empty[r][g % self.ns] for r in (0, 1)])]
+                    if i + 1 == n:
+                        self.pipe.append(("commit", self.qempty))
+                    t, g = t + 1, g + 1
+                if i >= AHEAD:
+                    v = t - 1 - (AHEAD if i < n else n + AHEAD - 1 - i)
+                    yield from wait(self.pfull[v & 1], v >> 1)
+                    yield from wait(self.full[g % self.ns], g // self.ns)
+                    if i == AHEAD and item:
+                        yield from wait(self.oread, item - 1)
+                    self.pipe += [("product", item), ("commit", [self.empty[r][g % self.ns] for r in (0, 1)]),
+                                  ("commit", [self.pdone[r][v & 1] for r in (0, 1)])]
+                    g += 1
+                yield None
+            self.pipe.append(("commit", self.odone))
+        self.over = True
+
+    def tensor(self):
+        while not (self.over and not self.pipe):
+            yield lambda: self.pipe or self.over
+            while self.pipe:
+                kind, what = self.pipe.pop(0)
+                if kind == "product":
+                    if any(self.reading.get(i) for i in range(what)):
+                        raise Fault("O overwritten before it was read")
+                else:
+                    for bar in self.rng.sample(what, len(what)):
+                        bar.arrive()
+                        yield None
+                yield None
+
+    def softmax(self, rank, wg, quarter):
+        t0 = u0 = told = zeroed = 0
+        pdone, box = self.pdone[rank], lambda u: (rank, quarter, u & 1)  # noqa: E731
+
+        def follow(u):
+            while self.m.get(box(u)) != u:
+                yield lambda: self.m.get(box(u)) == u
+
+        for item, (n, live0, live1, lo_edge, hi_edge) in enumerate(self.items):
+            idle = quarter >= (live1 if rank else live0)
+            if not idle:
+                self.reading.setdefault(item, set()).add((rank, wg, quarter))
+            for k in range((wg ^ t0) & 1, n, 2):
+                t = t0 + k
+                yield from wait(self.sfull[rank][wg], t >> 1)
+                yield None
+                self.sfree[wg].arrive(t >> 1)
+                yield None
+                if not idle:
+                    if k > 0:
+                        yield from follow(u0 + k - 1)
+                    self.m[box(u0 + k)] = u0 + k
+                    if k > 0 and self.rng.random() < 0.5:  # O is rescaled
+                        yield from wait(pdone[wg ^ 1], (t - 1) >> 1)
+                if t >= 2:
+                    yield from wait(pdone[wg], (t - 2) >> 1)
+                if (k == 0 and lo_edge) or (k == n - 1 and hi_edge):
+                    g = 2 * t0 + min(n, k + 1 + AHEAD) + k
+                    if rank == 0:
+                        yield from wait(self.full[g % self.ns], g // self.ns)
+                        if quarter == 0:
+                            self.vlanded[wg].arrive()
+                    else:
+                        yield from wait(self.vlanded[wg], zeroed)
+                        zeroed += 1
+                yield None
+                self.pfull[wg].arrive(t >> 1)
+            last = t0 + n - 1
+            if self.end == "item":
+                yield from wait(self.odone[rank], item)
+            else:  # the parity alone, as the hardware would
+                bar = pdone[last & 1]
+                while (bar.done & 1) == ((last >> 1) & 1):
+                    yield lambda: (bar.done & 1) != ((last >> 1) & 1)
+            if not idle:
+                if (last & 1) != wg:
+                    yield from follow(u0 + n - 1)
+                self.meet[rank][quarter].arrive(told)
+                yield from wait(self.meet[rank][quarter], told)
+                told += 1
+                u0 += n
+                yield None
+                yield None
+                self.reading[item].discard((rank, wg, quarter))
+            self.oread.arrive(item if self.end == "item" else None)
+            t0 += n
+            yield None
+
+    def run(self):
+        roles = [self.producer(0), self.producer(1), self.issuer(), self.tensor()]
+        roles += [self.softmax(r, w, q) for r in (0, 1) for w in (0, 1) for q in range(self.nq)]
+        ready = {x: None for x in roles}
+        speed = {x: 10.0 ** self.rng.uniform(-2, 1) for x in roles}
+        while ready:
+            can = [x for x, until in ready.items() if until is None or until()]
+            if not can:
+                raise Fault("standstill")
+            x = self.rng.choices(can, [speed[y] for y in can])[0]
+            try:
+                ready[x] = next(x)
+            except StopIteration:
+                del ready[x]
+
+
+def _items(rng, quarters=2):
+    return [(rng.choice([1, 1, 2, 2, 3, 3, 4, 5, 7]), rng.randint(1, quarters), rng.randint(0, quarters), rng.random() < 0.3,
+             rng.random() < 0.7) for _ in range(rng.randint(1, 7))]
+
+
+@pytest.mark.parametrize("slots,buffers", [(4, 1), (10, 2)])  # head_dim 256 and 128
+def test_every_wait_and_arrival_is_for_its_own_phase(slots, buffers):
+    for seed in range(300):
+        rng = random.Random(seed)
+        Pair(_items(rng), slots, buffers, rng).run()
+
+
+def test_model_sees_an_item_that_ends_a_phase_early():
+    # tiles 1, 2, 3 with idle quarters and an idle second CTA: a warp that owns
+    # only the middle tile, and waits for the last one's product by parity, may
+    # pass two phases early and then arrive twice in one phase of oread
+    seen = set()
+    for seed in range(600):
+        rng = random.Random(seed)
+        items = [(1, 2, 2, False, True), (2, 2, 2, False, True), (3, 1, 0, False, True), (2, 2, 0, False, True)]
+        try:
+            Pair(items, 10, 2, rng, end="tile").run()
+        except Fault as e:
+            seen.add(str(e))
+    assert "O overwritten before it was read" in seen, seen
