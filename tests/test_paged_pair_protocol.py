@@ -1,6 +1,7 @@
-"""The hand-offs of k_paged_attn_pair (mono-qwen27_b200/csrc/paged_attn.cu) as
-a model on the CPU: the roles of both CTAs as coroutines over barriers that know
-only a phase's parity, as the hardware's do, run in many random orders.
+"""The hand-offs of k_paged_attn_pair and k_paged_attn
+(mono-qwen27_b200/csrc/paged_attn.cu) as models on the CPU: a worker's roles as
+coroutines over barriers that know only a phase's parity, as the hardware's do,
+run in many random orders.
 
 An mbarrier wait names a parity, so one that comes two phases early passes at
 once.  The model counts phases, and calls a fault: a wait that passes for
@@ -179,9 +180,12 @@ class Pair:
             t0 += n
             yield None
 
+    def roles(self):
+        return [self.producer(0), self.producer(1), self.issuer(), self.tensor()] + [
+            self.softmax(r, w, q) for r in (0, 1) for w in (0, 1) for q in range(self.nq)]
+
     def run(self):
-        roles = [self.producer(0), self.producer(1), self.issuer(), self.tensor()]
-        roles += [self.softmax(r, w, q) for r in (0, 1) for w in (0, 1) for q in range(self.nq)]
+        roles = self.roles()
         ready = {x: None for x in roles}
         speed = {x: 10.0 ** self.rng.uniform(-2, 1) for x in roles}
         while ready:
@@ -195,6 +199,98 @@ class Pair:
                 del ready[x]
 
 
+class Single(Pair):
+    """One CTA: every softmax warp has half of each tile's positions."""
+
+    def __init__(self, items, slots, rng, quarters=2):
+        self.items, self.ns, self.rng, self.nq = items, slots, rng, quarters
+        n = 2 * quarters
+        self.full, self.empty = [Bar(2) for _ in range(slots)], [Bar(1) for _ in range(slots)]
+        self.qfull, self.sfull, self.sfree = Bar(n), Bar(1), Bar(n)
+        self.pfull, self.pdone = [Bar(n), Bar(n)], [Bar(1), Bar(1)]
+        self.meet = [Bar(2) for _ in range(quarters)]
+        self.pipe, self.reading, self.over = [], {}, False
+
+    def producer(self):
+        g = 0
+        for n, *_ in self.items:
+            for _ in range(2 * n):
+                if g >= self.ns:
+                    yield from wait(self.empty[g % self.ns], g // self.ns - 1)
+                self.full[g % self.ns].arrive()
+                yield None
+                self.full[g % self.ns].arrive()
+                g += 1
+
+    def issuer(self):
+        t0 = g = 0
+
+        def scores(t):
+            nonlocal g
+            if t > 0:
+                yield from wait(self.sfree, t - 1)
+            yield from wait(self.full[g % self.ns], g // self.ns)
+            self.pipe += [("commit", [self.sfull]), ("commit", [self.empty[g % self.ns]])]
+            g += 1
+
+        for item, (n, *_) in enumerate(self.items):
+            yield from wait(self.qfull, item)
+            yield from scores(t0)
+            if n > 1:
+                yield from scores(t0 + 1)
+            for i in range(n):
+                t = t0 + i
+                yield from wait(self.pfull[t & 1], t >> 1)
+                yield from wait(self.full[g % self.ns], g // self.ns)
+                self.pipe += [("product", item), ("commit", [self.empty[g % self.ns]]), ("commit", [self.pdone[t & 1]])]
+                g += 1
+                if i + 2 < n:
+                    yield from scores(t + 2)
+            t0 += n
+        self.over = True
+
+    def softmax(self, quarter):
+        t = g0 = told = 0
+        self.qfull.arrive(0)
+        for item, (n, live, _, lo_edge, hi_edge) in enumerate(self.items):
+            idle = quarter >= live
+            mine = object()
+            if not idle:
+                self.reading.setdefault(item, set()).add(mine)
+            for k in range(n):
+                yield from wait(self.sfull, t)
+                yield None
+                self.sfree.arrive(t)
+                if not idle:
+                    self.meet[quarter].arrive(told)
+                    yield from wait(self.meet[quarter], told)
+                    told += 1
+                    if k > 0 and self.rng.random() < 0.5:  # O is rescaled
+                        yield from wait(self.pdone[(t - 1) & 1], (t - 1) >> 1)
+                    if t >= 2:
+                        yield from wait(self.pdone[t & 1], (t - 2) >> 1)
+                if (k == 0 and lo_edge) or (k == n - 1 and hi_edge):
+                    g = g0 + (2 * n - 1 if k == n - 1 else 2 * k + 2)
+                    yield from wait(self.full[g % self.ns], g // self.ns)
+                yield None
+                self.pfull[t & 1].arrive(t >> 1)
+                t += 1
+            g0 += 2 * n
+            if item + 1 < len(self.items):
+                self.qfull.arrive(item + 1)
+            yield from wait(self.pdone[(t - 1) & 1], (t - 1) >> 1)
+            if not idle:
+                self.meet[quarter].arrive(told)
+                yield from wait(self.meet[quarter], told)
+                told += 1
+                yield None
+                self.reading[item].discard(mine)
+            yield None
+
+    def roles(self):
+        return [self.producer(), self.issuer(), self.tensor()] + [self.softmax(q) for q in range(self.nq) for _ in (0, 1)]
+
+
 def _items(rng, quarters=2):
     return [(rng.choice([1, 1, 2, 2, 3, 3, 4, 5, 7]), rng.randint(1, quarters), rng.randint(0, quarters), rng.random() < 0.3,
              rng.random() < 0.7) for _ in range(rng.randint(1, 7))]
@@ -205,6 +301,13 @@ def test_every_wait_and_arrival_is_for_its_own_phase(slots, buffers):
     for seed in range(300):
         rng = random.Random(seed)
         Pair(_items(rng), slots, buffers, rng).run()
+
+
+@pytest.mark.parametrize("slots", [6, 12])  # head_dim 128 and 256, 64
+def test_the_same_for_single_ctas(slots):
+    for seed in range(300):
+        rng = random.Random(seed)
+        Single(_items(rng), slots, rng).run()
 
 
 def test_model_sees_an_item_that_ends_a_phase_early():
