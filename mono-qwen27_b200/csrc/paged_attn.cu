@@ -1627,7 +1627,10 @@ bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const v
     if (kv->page_stride >= 1ll << 39) return paged_fail(err, err_cap, "%s: page_stride (%lld) too large", what, kv->page_stride);
     const int ctas = pa_ctas(), G = n_q / kv->n_kv;
     if (ctas < 2) return paged_fail(err, err_cap, "%s: no CUDA device", what);
-    const AttnArgs a = {*kv, *batch, q, out, lse, q_stride, out_stride, n_q, window > 0 ? window : 0, scale,
+    // a window of all that a row of the table holds is none, so that the kernels'
+    // differences of positions (2^30 at most on either side) stay in 32 bits
+    if (window < 0 || window >= kv->n_cols * kv->page_size) window = 0;
+    const AttnArgs a = {*kv, *batch, q, out, lse, q_stride, out_stride, n_q, window, scale,
                         (PaItem *)scratch, (float *)((char *)scratch + PA_MAX_CTAS * sizeof(PaItem)), status_ptr_current()};
     // Pairs of CTAs when a sequence has rows for one and a half, on average.  With
     // 128, 192, 256, 512 rows a sequence, microseconds by single CTAs and by pairs

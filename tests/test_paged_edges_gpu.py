@@ -87,3 +87,22 @@ def test_items_of_one_two_and_three_tiles_with_idle_quarters(torch, m27b, hd, dt
         again, lse2 = _run(torch, m27b, c, q, cu)
         assert torch.equal(again, out) and torch.equal(lse2, lse)
     assert m27b.device_status() == 0
+
+
+@pytest.mark.parametrize("hd,q_lens,kv_lens", [(64, [13, 1, 40], [3, 90, 20]), (128, [13, 1], [3, 90]), (128, [300, 90], [100, 70]),
+                                               (256, [300, 150], [290, 150])])
+def test_a_window_of_any_size(torch, m27b, hd, q_lens, kv_lens):
+    # a window that reaches past the cache is none, up to the type's end, also
+    # where a sequence has fewer positions than new tokens
+    c = Cache(torch, m27b, kv_lens, 16, 2, hd, "bf16", 52)
+    q = torch.randn(sum(q_lens), 8, hd, device="cuda").bfloat16()
+    cu = _cu(torch, q_lens)
+    want = _run(torch, m27b, c, q, cu)
+    at = 0
+    for b, n in enumerate(q_lens):
+        _close(torch, want[0][at:at + n], want[1][at:at + n], _attend(torch, q[at:at + n], *_seq(torch, c, b), hd ** -0.5, 0), "bf16")
+        at += n
+    for window in (2 ** 31 - 1, 2 ** 31 - 200, 2 ** 30, c.tab.shape[1] * 16, -1):
+        got = _run(torch, m27b, c, q, cu, window=window)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), window
+    assert m27b.device_status() == 0
