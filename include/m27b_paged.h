@@ -119,7 +119,8 @@ typedef struct M27BHeads {
  * to q_out (q_out + t * q_out_stride + h * head_dim), k and the unrotated v to
  * the token's slot in the cache.  All arithmetic in fp32.  q_out may be q
  * itself when the types agree.  n_q = 0 appends only.  A token whose position
- * or page is out of range is left out (status 6). */
+ * or page is out of range is left out (status 6).  In f16 a value above 65504
+ * becomes an infinity, and rows that attend to it may become NaN. */
 M27B_API bool m27b_rope_append(const M27BPagedKV *kv, const M27BPagedBatch *batch, const M27BRope *rope,
                                const M27BHeads *heads, void *q_out, long long q_out_stride, cudaStream_t stream,
                                char *err, size_t err_cap);
@@ -140,7 +141,8 @@ M27B_API size_t m27b_paged_attn_scratch_bytes(int n_q, int n_kv, int head_dim);
  * gets zeros and -inf.  Scores, softmax statistics and sums are fp32; the
  * weights are rounded to the cache's type for their product with V.  Slots
  * that no row of the sequence sees may hold anything, infinities and NaN
- * included; a position that the sequence holds must be finite. */
+ * included; a position that the sequence holds must be finite.  A row of q with
+ * a NaN gets NaN in out and lse, and so does a row that sees one in K. */
 M27B_API bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const void *q, long long q_stride,
                               int n_q, float scale, int window, void *out, long long out_stride, float *lse,
                               void *scratch, cudaStream_t stream, char *err, size_t err_cap);

@@ -547,7 +547,8 @@ M27B_DI void transpose4(uint4 (&y)[4]) {
 // The end of an item in this worker's run: this thread's part of its row's O
 // (columns [part HD / PARTS, ..) of TMEM at `o`) to the output, or, if the worker
 // has a part of the item only, O, m and l to its record.  `tok`: the first
-// token row of the CTA's rows; `any`: there were tiles (else O is 0).
+// token row of the CTA's rows; `any`: there were tiles (else O is 0).  l is 0
+// for a row that saw nothing, whose O is not read, and NaN where scores were.
 template <int HD, bool BF, int PARTS, class Walk>
 M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me, int cta, int tok, int G, int rows, int row,
                       int part, bool any, float m, float l, uint32_t o, PaItem &tail) {
@@ -557,8 +558,8 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
     const long long at = tok + row / G;
     if (w.whole()) {
         if (idle) return;
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        const bool nothing = __any_sync(0xffffffffu, !(l > 0.0f));  // some row's O is not to be read
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const bool nothing = __any_sync(0xffffffffu, l == 0.0f);  // some row's O is not to be read
         // where quadruple row & 3 of 32 columns of rows (row & ~3) .. + 3 goes
         uint16_t *to[4];
         int i = (row & ~3) / G, g = (row & ~3) - i * G;
@@ -576,7 +577,7 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
                 tmem_ld32(o + part * COLS + 32 * x, v);
                 tmem_wait_ld();
             }
-            if (nothing && !(l > 0.0f))
+            if (nothing && l == 0.0f)
 #pragma unroll
                 for (int e = 0; e < 32; ++e) v[e] = 0u;
             // four quadruples of 16 bits; then lane 4 g + j holds quadruple j of rows
@@ -596,7 +597,7 @@ M27B_DI void pa_write(const AttnArgs &a, const Walk &w, const PaRun &run, int me
                 if (to[r]) *(uint4 *)(to[r] + 32 * x) = y[r];
         }
         if (live && a.lse && part == 0)
-            a.lse[at * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
+            a.lse[at * a.n_q + h] = l != 0.0f ? 0.69314718055994530942f * (m + log2f(l)) : -INFINITY;
     } else {
         // the item begins with worker c0 and ends with c1
         const long long U = w.u - w.off;
@@ -1426,7 +1427,7 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
             for (int v = 0; v < 8; ++v) o[v] *= f0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                if (ml[q].x == -INFINITY) continue;  // the part saw nothing (its O may be anything)
+                if (ml[q].y == 0.0f) continue;  // the part saw nothing (its O may be anything)
                 const float f = ex2(ml[q].x - ref);
                 l = fmaf(f, ml[q].y, l);
 #pragma unroll
@@ -1450,7 +1451,7 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
             for (int v = 0; v < 8; ++v) o[v] += __shfl_xor_sync(0xffffffffu, o[v], d);
         }
         if (p != 0 || e0 + (int)threadIdx.x / SP >= n) continue;
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
         uint32_t y[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) y[v] = Half16<BF>::down(o[2 * v] * inv, o[2 * v + 1] * inv);
@@ -1458,7 +1459,7 @@ M27B_DI void pa_join(const AttnArgs &a, const PaItem &it, int stride) {
         const int h = it.j * G + row % G;
         *(uint4 *)((uint16_t *)a.out + tok * a.out_stride + (long long)h * HD + 8 * d8) = make_uint4(y[0], y[1], y[2], y[3]);
         if (d8 == 0 && a.lse)
-            a.lse[tok * a.n_q + h] = l > 0.0f ? 0.69314718055994530942f * (mx + log2f(l)) : -INFINITY;
+            a.lse[tok * a.n_q + h] = l != 0.0f ? 0.69314718055994530942f * (mx + log2f(l)) : -INFINITY;
     }
 }
 

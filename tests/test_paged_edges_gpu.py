@@ -106,3 +106,38 @@ def test_a_window_of_any_size(torch, m27b, hd, q_lens, kv_lens):
         got = _run(torch, m27b, c, q, cu, window=window)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), window
     assert m27b.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hd,q_lens,kv_lens", [
+    (64, [1, 3, 40], [500, 3, 41]),           # whole items
+    (256, [1, 1], [9000, 40]),                # an item over many workers, joined
+    (128, [300, 150], [300, 150]),            # pairs
+    (128, [100], [6000]), (256, [140], [4000]),  # pairs, joined
+])
+def test_a_nan_in_q_stays_one(torch, m27b, dtype, hd, q_lens, kv_lens):
+    # a row whose scores are NaN is NaN, not the zeros of a row that sees nothing;
+    # the other rows are as without it
+    c = Cache(torch, m27b, kv_lens, 16, 2, hd, dtype, 53)
+    q = torch.randn(sum(q_lens), 4, hd, device="cuda").to(c.k.dtype)
+    cu = _cu(torch, q_lens)
+    out, lse = _run(torch, m27b, c, q, cu)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[-1, 2] = bad[len(q) // 2, 0] = True
+    q[bad.nonzero()[:, 0], bad.nonzero()[:, 1], hd // 3] = float("nan")
+    got, got_l = _run(torch, m27b, c, q, cu)
+    assert bool(torch.isnan(got[bad]).all()) and bool(torch.isnan(got_l[bad]).all())
+    assert torch.equal(got[~bad], out[~bad]) and torch.equal(got_l[~bad], lse[~bad])
+    assert m27b.device_status() == 0
+
+
+@pytest.mark.parametrize("hd,kv_len", [(64, 700), (128, 9000)])
+def test_a_nan_key_that_a_row_sees_is_not_an_empty_row(torch, m27b, hd, kv_len):
+    c = Cache(torch, m27b, [kv_len, 200], 16, 2, hd, "bf16", 54)
+    q = torch.randn(2, 4, hd, device="cuda").bfloat16()
+    cu = _cu(torch, [1, 1])
+    out, lse = _run(torch, m27b, c, q, cu)
+    c.k[int(c.tab[0, 10]), 3, 1, 5] = float("nan")  # kv head 1: query heads 2 and 3
+    got, got_l = _run(torch, m27b, c, q, cu)
+    assert bool(torch.isnan(got[0, 2:]).all()) and bool(torch.isnan(got_l[0, 2:]).all())
+    assert torch.equal(got[0, :2], out[0, :2]) and torch.equal(got[1], out[1]) and torch.equal(got_l[1], lse[1])
