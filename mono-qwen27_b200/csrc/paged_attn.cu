@@ -55,8 +55,13 @@
 // Q K of tile t + 2, P V of tile t + 1, ...
 //
 // m moves only when the running maximum has grown by more than 2^8 since it
-// was set: weights then stay below 2^8 (fp32 sums, and far from the 16-bit
-// types' limits), and O in TMEM is rescaled on few tiles.
+// was set, so that O in TMEM is rescaled on few tiles.  For bf16 it is set to
+// the maximum: weights stay below 2^8, far from the type's limits.  For f16 it is
+// set 7 below: weights stay below 2^15 (f16 ends at 2^16), and the largest is at
+// least 2^7, so that those which f16 holds with fewer than 11 bits (below 2^-14,
+// with an absolute error of 2^-25) are below 2^-21 of it and their errors at
+// most 2^-32 of it each.  Set to the maximum, a weight of 2^-25 of the largest is
+// lost, and 40000 such positions beside a large one are 0.1 % of the sum.
 //
 // Rows of a V tile that no row of the sequence sees may hold anything: their
 // weights are 0, but 0 * NaN is not, so the softmax warps overwrite them with
@@ -93,7 +98,8 @@ constexpr int PA_ROWS = 128;
 constexpr int PA_SOFTMAX = 8;  // softmax warps: two for each 32 rows, each with half of a tile's positions
 constexpr int PA_PRODUCER = PA_SOFTMAX, PA_ISSUER = PA_SOFTMAX + 1;
 constexpr int PA_THREADS = (PA_SOFTMAX + 2) * 32;
-constexpr float PA_SLACK = 8.0f;  // growth of the maximum (log2) before m follows
+template <bool BF> constexpr float PA_BELOW = BF ? 0.0f : 7.0f;     // m is set this far below the maximum (log2)
+template <bool BF> constexpr float PA_SLACK = 8.0f + PA_BELOW<BF>;  // the maximum above m before m follows
 
 template <int HD> struct PaPlan {
     static constexpr int KT = HD == 256 ? 64 : 128;  // positions per key tile
@@ -837,8 +843,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     const float mine = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     if (!(ok = other(mine, theirs))) break;
                     const float top = c * fmaxf(mine, theirs);
-                    if (__any_sync(0xffffffffu, top > m + PA_SLACK)) {
-                        const float to = top > m + PA_SLACK ? top : m;
+                    if (__any_sync(0xffffffffu, top > m + PA_SLACK<BF>)) {
+                        const float to = top > m + PA_SLACK<BF> ? top - PA_BELOW<BF> : m;
                         const float f = m == -INFINITY ? 1.0f : ex2(m - to);
                         m = to;
                         l *= f;
@@ -1273,7 +1279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     // the other warps' m after the tile before, and ours
                     float before = -INFINITY;
                     if (k > 0 && !(ok = follow(u0 + k - 1, before))) break;
-                    const float now = top > before + PA_SLACK ? top : before;
+                    const float now = top > before + PA_SLACK<BF> ? top - PA_BELOW<BF> : before;
                     publish(u0 + k, now);
                     if (m != now) {
                         l *= m == -INFINITY ? 0.0f : ex2(m - now);

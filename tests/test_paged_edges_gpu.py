@@ -141,3 +141,33 @@ def test_a_nan_key_that_a_row_sees_is_not_an_empty_row(torch, m27b, hd, kv_len):
     got, got_l = _run(torch, m27b, c, q, cu)
     assert bool(torch.isnan(got[0, 2:]).all()) and bool(torch.isnan(got_l[0, 2:]).all())
     assert torch.equal(got[0, :2], out[0, :2]) and torch.equal(got[1], out[1]) and torch.equal(got_l[1], lse[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,n_seq,n_tok,group", [(64, 200, 1, 1), (128, 200, 1, 2), (256, 200, 1, 2), (128, 90, 12, 16), (256, 90, 12, 16)])
+@pytest.mark.parametrize("sink", ["first", "last"])
+def test_many_small_weights_beside_a_large_one(torch, m27b, dtype, hd, n_seq, n_tok, group, sink):
+    # one position with nearly all of the weight and a value of 0, and 40000 whose
+    # weights are 2^-25.25 to 2^-26 of its: the result is what these add up to.  All rows of the
+    # table hold the same pages; with so many sequences no worker has less than
+    # about half of one.
+    n, ps = 40000, 64
+    g = torch.Generator(device="cuda").manual_seed(55)
+    c = Cache(torch, m27b, [n], ps, 1, hd, dtype, 56)
+    d = torch.randint(25 * 8 + 2, 26 * 8 + 1, (n,), generator=g, device="cuda") / 8  # exact in both types
+    key, val = torch.zeros(n, 1, hd, device="cuda"), 0.5 + torch.rand(n, 1, hd, generator=g, device="cuda")
+    at = 0 if sink == "first" else n - n_tok
+    d[at] = 0
+    key[:, 0, 0], val[at] = -d, 0.0
+    ids = c.table[0, :P.cdiv(n, ps)].long()
+    c.k[ids], c.v[ids] = key.to(c.k.dtype).view(-1, ps, 1, hd), val.to(c.v.dtype).view(-1, ps, 1, hd)
+    q = torch.zeros(n_seq * n_tok, group, hd, device="cuda", dtype=c.k.dtype)
+    q[..., 0] = 1.0
+    kv = m27b.PagedKV(c.k, c.v, c.table.repeat(n_seq, 1).contiguous())
+    lens, scale = torch.full((n_seq,), n, dtype=torch.int32, device="cuda"), float(np.log(2.0))
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    m27b.paged_attn(kv, q, _cu(torch, [n_tok] * n_seq), lens, out, m27b.paged_attn_scratch(group, 1, hd), scale=scale, lse=lse)
+    want = _attend(torch, q[:n_tok], *_seq(torch, c, 0), scale, 0)
+    for b in range(0, n_seq, 13):
+        _close(torch, out[b * n_tok:(b + 1) * n_tok], lse[b * n_tok:(b + 1) * n_tok], want, dtype)
+    assert m27b.device_status() == 0
