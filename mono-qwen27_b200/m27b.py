@@ -999,8 +999,10 @@ def paged_attn(kv, q, cu_q, lens, out, scratch, scale=None, window=0, lse=None, 
     qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt)
     op, os_ = _token_heads(out, "out", n_tok, n_q, hd, dt)
     L = _paged_lib()
-    if not scratch.is_cuda or scratch.numel() < L.m27b_paged_attn_scratch_bytes(n_q, kv.n_kv, hd):
-        raise M27BError("paged_attn: scratch is too small for these heads (use paged_attn_scratch)")
+    need = L.m27b_paged_attn_scratch_bytes(n_q, kv.n_kv, hd)
+    # contiguous: an expanded tensor has more values than memory
+    if not scratch.is_cuda or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < need:
+        raise M27BError(f"paged_attn: scratch must be {need} contiguous bytes on the device (use paged_attn_scratch)")
     lp = None
     if lse is not None:
         if lse.numel() != n_tok * n_q or not _f32(lse):
