@@ -852,9 +852,9 @@ def _paged_type(dtype):
     return t
 
 
-def _f32(t):
-    """A contiguous fp32 device tensor?"""
-    return t.is_cuda and _paged_type(t.dtype) == F32 and t.is_contiguous()
+def _f32(t, dev):
+    """A contiguous fp32 tensor on device `dev`?"""
+    return t.get_device() == dev and _paged_type(t.dtype) == F32 and t.is_contiguous()
 
 
 # A decode step makes these calls once per layer on a few rows, so what they
@@ -871,27 +871,34 @@ def _err():
         return _tls.err
 
 
-def _raw_stream(stream):
-    if stream is not None:
-        return stream.cuda_stream
+def _raw_stream(stream, dev):
+    """The handle of `stream` or the current one.  The C entries work on the
+    current device, so that has to be the tensors' (`dev`), and the stream's."""
     import torch
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    cur = torch._C._cuda_getDevice()
+    if cur != dev or (stream is not None and stream.device_index != dev):
+        raise M27BError(f"paged cache: the tensors are on device {dev}, the current device is {cur}"
+                        + ("" if stream is None else f", the stream's {stream.device_index}"))
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
 
 
-def _int32(t, what, n=0):
-    """The data pointer of a contiguous device int32 tensor (0 for None)."""
+def _int32(t, what, n=0, dev=None):
+    """The data pointer of a contiguous int32 tensor on device `dev` (None: any; 0 for no tensor)."""
     if t is None:
         return 0
-    if not t.is_cuda or _paged_type(t.dtype) != I32 or t.numel() < n or not t.is_contiguous():
+    d = t.get_device()
+    if d < 0 or _paged_type(t.dtype) != I32 or t.numel() < n or not t.is_contiguous():
         raise M27BError(f"{what} must be a contiguous int32 device tensor" + (f" of at least {n} values" if n else ""))
+    if dev is not None and d != dev:
+        raise M27BError(f"{what} is on device {d}, the cache on device {dev}")
     return t.data_ptr()
 
 
-def _token_heads(t, what, n_tok, n_head, head_dim, dtype):
-    """(pointer, token stride) of [n_tok, n_head, head_dim] rows whose heads are contiguous."""
-    if t.shape != (n_tok, n_head, head_dim) or t.dtype != dtype or not t.is_cuda:
-        raise M27BError(f"{what} must be a device tensor [{n_tok}, {n_head}, {head_dim}] of {dtype} "
-                        f"(got {list(t.shape)} of {t.dtype})")
+def _token_heads(t, what, n_tok, n_head, head_dim, dtype, dev):
+    """(pointer, token stride) of [n_tok, n_head, head_dim] rows on device `dev` whose heads are contiguous."""
+    if t.shape != (n_tok, n_head, head_dim) or t.dtype != dtype or t.get_device() != dev:
+        raise M27BError(f"{what} must be a tensor [{n_tok}, {n_head}, {head_dim}] of {dtype} on device {dev} "
+                        f"(got {list(t.shape)} of {t.dtype} on {t.get_device()})")
     s = t.stride()
     if s[2] != 1 or (s[1] != head_dim and n_head > 1):
         raise M27BError(f"{what}: a token's heads must be contiguous (strides {s})")
@@ -916,8 +923,10 @@ class PagedKV:
         if table.dim() != 2:
             raise M27BError("PagedKV: table must be [n_rows, n_cols]")
         self.k, self.v, self.table = k, v, table
-        self.n_kv, self.head_dim, self.dtype = n_kv, head_dim, k.dtype
-        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _int32(table, "table"), _paged_type(k.dtype), n_pages, page_size,
+        self.n_kv, self.head_dim, self.dtype, self.dev = n_kv, head_dim, k.dtype, k.get_device()
+        if v.get_device() != self.dev:
+            raise M27BError(f"PagedKV: k is on device {self.dev}, v on device {v.get_device()}")
+        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _int32(table, "table", 0, self.dev), _paged_type(k.dtype), n_pages, page_size,
                           n_kv, head_dim, table.shape[0], table.shape[1],
                           s[0] if n_pages > 1 else page_size * n_kv * head_dim)
         self._ref = ctypes.byref(self.c)
@@ -928,8 +937,9 @@ def _batch(kv, cu_q, lens, rows, n_tok):
     n_seq = cu_q.numel() - 1
     if n_seq < 0:
         raise M27BError("cu_q needs n_seq + 1 values")
-    return _PagedBatch.pack(_int32(cu_q, "cu_q"), _int32(lens, "lens", kv.c.n_rows if rows is not None else n_seq),
-                            _int32(rows, "rows", n_seq), n_seq, n_tok)
+    return _PagedBatch.pack(_int32(cu_q, "cu_q", 0, kv.dev),
+                            _int32(lens, "lens", kv.c.n_rows if rows is not None else n_seq, kv.dev),
+                            _int32(rows, "rows", n_seq, kv.dev), n_seq, n_tok)
 
 
 def rope_table(n_pos, n_rot, theta, kind=ROPE_NONE, factor=1.0, original_ctx=0, beta_fast=32.0, beta_slow=1.0,
@@ -941,8 +951,8 @@ def rope_table(n_pos, n_rot, theta, kind=ROPE_NONE, factor=1.0, original_ctx=0, 
     out = torch.empty(n_pos, n_rot // 2, 2, dtype=torch.float32, device=device)
     s = _RopeScaling(kind, factor, original_ctx, beta_fast, beta_slow, attn_factor)
     err = ctypes.create_string_buffer(ERR_CAP)
-    _check(_paged_lib().m27b_rope_table(_ptr(out), n_pos, n_rot, theta, ctypes.byref(s), _stream(stream), err, ERR_CAP),
-           err, "m27b_rope_table")
+    _check(_paged_lib().m27b_rope_table(_ptr(out), n_pos, n_rot, theta, ctypes.byref(s),
+                                        _raw_stream(stream, out.get_device()), err, ERR_CAP), err, "m27b_rope_table")
     return out
 
 
@@ -953,27 +963,27 @@ def rope_append(kv, q, k, v, cu_q, lens, rope, q_out, interleaved=False, q_norm=
     the cache (m27b_rope_append).  cu_q [n_seq + 1]: each sequence's token
     rows; lens: positions of each table row, the new ones included; rope: a
     table of rope_table.  q may be None (append only)."""
-    dt, n_kv, hd = k.dtype, kv.n_kv, kv.head_dim
+    dt, n_kv, hd, dev = k.dtype, kv.n_kv, kv.head_dim, kv.dev
     n_tok = k.shape[0]
-    kp, ks = _token_heads(k, "k", n_tok, n_kv, hd, dt)
-    vp, vs = _token_heads(v, "v", n_tok, n_kv, hd, dt)
+    kp, ks = _token_heads(k, "k", n_tok, n_kv, hd, dt, dev)
+    vp, vs = _token_heads(v, "v", n_tok, n_kv, hd, dt, dev)
     n_q = qp = op = qs = os_ = 0
     if q is not None:
         n_q = q.shape[1]
-        qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt)
-        op, os_ = _token_heads(q_out, "q_out", n_tok, n_q, hd, kv.dtype)
+        qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt, dev)
+        op, os_ = _token_heads(q_out, "q_out", n_tok, n_q, hd, kv.dtype, dev)
     n_pos, half, two = rope.shape
-    if two != 2 or not _f32(rope):
-        raise M27BError("rope must be an fp32 table [n_pos, n_rot / 2, 2]")
-    if (q_norm is not None and (q_norm.numel() != hd or not _f32(q_norm))) or \
-            (k_norm is not None and (k_norm.numel() != hd or not _f32(k_norm))):
-        raise M27BError(f"q_norm and k_norm must be {hd} fp32 values on the device")
+    if two != 2 or not _f32(rope, dev):
+        raise M27BError(f"rope must be an fp32 table [n_pos, n_rot / 2, 2] on device {dev}")
+    if (q_norm is not None and (q_norm.numel() != hd or not _f32(q_norm, dev))) or \
+            (k_norm is not None and (k_norm.numel() != hd or not _f32(k_norm, dev))):
+        raise M27BError(f"q_norm and k_norm must be {hd} fp32 values on device {dev}")
     bt = _batch(kv, cu_q, lens, rows, n_tok)
-    rp = _Rope.pack(rope.data_ptr(), n_pos, 2 * half, 1 if interleaved else 0, _int32(positions, "positions", n_tok))
+    rp = _Rope.pack(rope.data_ptr(), n_pos, 2 * half, 1 if interleaved else 0, _int32(positions, "positions", n_tok, dev))
     h = _Heads.pack(qp, kp, vp, qs, ks, vs, _paged_type(dt), n_q, 0 if q_norm is None else q_norm.data_ptr(),
                     0 if k_norm is None else k_norm.data_ptr(), eps)
     err = _err()
-    if not _paged_lib().m27b_rope_append(kv._ref, bt, rp, h, op, os_, _raw_stream(stream), err,
+    if not _paged_lib().m27b_rope_append(kv._ref, bt, rp, h, op, os_, _raw_stream(stream, dev), err,
                                          ERR_CAP):
         _check(False, err, "m27b_rope_append")
     return q_out
@@ -994,24 +1004,24 @@ def paged_attn(kv, q, cu_q, lens, out, scratch, scale=None, window=0, lse=None, 
     lens - 1; window > 0 limits a token to the last `window` positions; lse
     [n_tok, n_q] fp32 receives the log sum of exponentials.  scale defaults to
     1 / sqrt(hd)."""
-    hd, dt = kv.head_dim, kv.dtype
+    hd, dt, dev = kv.head_dim, kv.dtype, kv.dev
     n_tok, n_q, _ = q.shape
-    qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt)
-    op, os_ = _token_heads(out, "out", n_tok, n_q, hd, dt)
+    qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt, dev)
+    op, os_ = _token_heads(out, "out", n_tok, n_q, hd, dt, dev)
     L = _paged_lib()
     need = L.m27b_paged_attn_scratch_bytes(n_q, kv.n_kv, hd)
     # contiguous: an expanded tensor has more values than memory
-    if not scratch.is_cuda or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < need:
-        raise M27BError(f"paged_attn: scratch must be {need} contiguous bytes on the device (use paged_attn_scratch)")
+    if scratch.get_device() != dev or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < need:
+        raise M27BError(f"paged_attn: scratch must be {need} contiguous bytes on device {dev} (use paged_attn_scratch)")
     lp = None
     if lse is not None:
-        if lse.numel() != n_tok * n_q or not _f32(lse):
-            raise M27BError(f"lse must be {n_tok} x {n_q} fp32 values on the device")
+        if lse.numel() != n_tok * n_q or not _f32(lse, dev):
+            raise M27BError(f"lse must be {n_tok} x {n_q} fp32 values on device {dev}")
         lp = lse.data_ptr()
     bt = _batch(kv, cu_q, lens, rows, n_tok)
     err = _err()
     if not L.m27b_paged_attn(kv._ref, bt, qp, qs, n_q, hd ** -0.5 if scale is None else scale, window, op, os_, lp,
-                             scratch.data_ptr(), _raw_stream(stream), err, ERR_CAP):
+                             scratch.data_ptr(), _raw_stream(stream, dev), err, ERR_CAP):
         _check(False, err, "m27b_paged_attn")
     return out
 
@@ -1033,17 +1043,17 @@ class PageSet:
             raise M27BError("PageSet: table must be [n_rows, n_cols], lens [n_rows]")
         self.table, self.ref, self.lens, self.page_size = table, ref, lens, page_size
         self.pools = list(pool) if isinstance(pool, (list, tuple)) else [pool]
-        n_pages = ref.numel()
+        n_pages, self.dev = ref.numel(), ref.get_device()
         arr = []
         for p in self.pools:
-            if p.dim() < 3 or p.shape[1] != n_pages or not p.is_cuda or not p[0, 0].is_contiguous():
-                raise M27BError(f"PageSet: a pool is [n_planes, {n_pages}, ...] on the device, its pages contiguous")
+            if p.dim() < 3 or p.shape[1] != n_pages or p.get_device() != self.dev or not p[0, 0].is_contiguous():
+                raise M27BError(f"PageSet: a pool is [n_planes, {n_pages}, ...] on ref's device ({self.dev}), its pages contiguous")
             es = p.element_size()
             page_bytes = p[0, 0].numel() * es
             arr.append(_PagePool(p.data_ptr(), p.shape[0], p.stride(0) * es if p.shape[0] > 1 else 0,
                                  p.stride(1) * es if n_pages > 1 else page_bytes, page_bytes))
         self._pools = (_PagePool * len(arr))(*arr)
-        self.c = _Pages(_int32(ref, "ref"), _int32(table, "table"), _int32(lens, "lens"), n_pages, page_size,
+        self.c = _Pages(_int32(ref, "ref"), _int32(table, "table", 0, self.dev), _int32(lens, "lens", 0, self.dev), n_pages, page_size,
                         table.shape[0], table.shape[1])
         self._ref = ctypes.byref(self.c)
         self.max_requests = table.shape[0] if max_requests is None else max_requests
@@ -1062,14 +1072,14 @@ class PageSet:
 
     def _call(self, name, *args, stream=None):
         err = _err()
-        if not getattr(_paged_lib(), name)(*args, _raw_stream(stream), err, ERR_CAP):
+        if not getattr(_paged_lib(), name)(*args, _raw_stream(stream, self.dev), err, ERR_CAP):
             _check(False, err, name)
 
     def _requests(self, a, b, names):
         n = a.numel()
         if n > self.max_requests or (b is not None and b.numel() != n):
             raise M27BError(f"PageSet: {names}: at most {self.max_requests} requests, as many of each")
-        return _int32(a, names), _int32(b, names), n
+        return _int32(a, names, 0, self.dev), _int32(b, names, 0, self.dev), n
 
     def resize(self, rows, new_lens, stream=None):
         """Set the rows' lengths (m27b_pages_resize)."""
@@ -1085,19 +1095,19 @@ class PageSet:
 
     def free(self, rows, stream=None):
         """Empty the rows (m27b_pages_free)."""
-        self._call("m27b_pages_free", self._ref, _int32(rows, "rows"), rows.numel(), stream=stream)
+        self._call("m27b_pages_free", self._ref, _int32(rows, "rows", 0, self.dev), rows.numel(), stream=stream)
 
     def compact(self, n_live=None, stream=None):
         """Move the pages in use to the lowest ids (m27b_pages_compact); n_live, an int32 device tensor, receives their number."""
-        self._call("m27b_pages_compact", self._ref, self._pools, len(self._pools), _int32(n_live, "n_live", 1),
+        self._call("m27b_pages_compact", self._ref, self._pools, len(self._pools), _int32(n_live, "n_live", 1, self.dev),
                    self._scratch.data_ptr(), stream=stream)
 
     def copy(self, src, dst, stream=None):
         """Copy page src[i] to page dst[i] in every plane (m27b_pages_copy)."""
         if src.numel() != dst.numel():
             raise M27BError("PageSet: src and dst need as many pages")
-        self._call("m27b_pages_copy", self._pools, len(self._pools), self.c.n_pages, _int32(src, "src"), _int32(dst, "dst"),
-                   src.numel(), stream=stream)
+        self._call("m27b_pages_copy", self._pools, len(self._pools), self.c.n_pages, _int32(src, "src", 0, self.dev),
+                   _int32(dst, "dst", 0, self.dev), src.numel(), stream=stream)
 
     def check(self):
         """Raise if a request was refused since the last check (reads the device)."""
