@@ -905,6 +905,16 @@ def _token_heads(t, what, n_tok, n_head, head_dim, dtype, dev):
     return t.data_ptr(), s[0] if n_tok > 1 else n_head * head_dim
 
 
+def _no_grad(what, *tensors):
+    """As torch's functions with out=: results in given buffers carry no gradient."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            import torch
+            if torch.is_grad_enabled():
+                raise M27BError(f"{what} has no backward pass, and a tensor given to it requires grad (use torch.no_grad())")
+            return
+
+
 class PagedKV:
     """One layer's pools of a paged cache, with the page table.
 
@@ -962,9 +972,10 @@ def rope_append(kv, q, k, v, cu_q, lens, rope, q_out, interleaved=False, q_norm=
     and k [n_tok, n_kv, hd]; q goes to q_out, k and v to the tokens' slots of
     the cache (m27b_rope_append).  cu_q [n_seq + 1]: each sequence's token
     rows; lens: positions of each table row, the new ones included; rope: a
-    table of rope_table.  q may be None (append only)."""
+    table of rope_table.  q may be None (append only).  No backward pass."""
     dt, n_kv, hd, dev = k.dtype, kv.n_kv, kv.head_dim, kv.dev
     n_tok = k.shape[0]
+    _no_grad("rope_append", q, k, v, q_norm, k_norm)
     kp, ks = _token_heads(k, "k", n_tok, n_kv, hd, dt, dev)
     vp, vs = _token_heads(v, "v", n_tok, n_kv, hd, dt, dev)
     n_q = qp = op = qs = os_ = 0
@@ -1003,9 +1014,10 @@ def paged_attn(kv, q, cu_q, lens, out, scratch, scale=None, window=0, lse=None, 
     (m27b_paged_attn): one token or many per sequence, the newest at position
     lens - 1; window > 0 limits a token to the last `window` positions; lse
     [n_tok, n_q] fp32 receives the log sum of exponentials.  scale defaults to
-    1 / sqrt(hd)."""
+    1 / sqrt(hd).  No backward pass."""
     hd, dt, dev = kv.head_dim, kv.dtype, kv.dev
     n_tok, n_q, _ = q.shape
+    _no_grad("paged_attn", q, kv.k, kv.v)
     qp, qs = _token_heads(q, "q", n_tok, n_q, hd, dt, dev)
     op, os_ = _token_heads(out, "out", n_tok, n_q, hd, dt, dev)
     L = _paged_lib()

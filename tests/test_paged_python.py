@@ -110,3 +110,19 @@ def test_another_current_device_or_stream(m27b, monkeypatch):
     for call in (lambda: _attn(torch, m27b, stream=Stream), lambda: _rope(torch, m27b, stream=Stream)):
         with pytest.raises(m27b.M27BError, match="the stream's 1"):
             call()
+
+
+def test_tensors_that_require_grad(m27b, monkeypatch):
+    # the results would carry no gradient without a word
+    torch = _torch()
+    bf, f32 = torch.bfloat16, torch.float32
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)  # what no_grad lets through ends at the device
+    want = lambda shape, dt: Dev(torch, shape, dt, grad=True)  # noqa: E731
+    for call, kw in ((_attn, dict(q=want((3, 4, 64), bf))), (_attn, dict(k=want((4, 16, 2, 64), bf))),
+                     (_attn, dict(v=want((4, 16, 2, 64), bf))), (_rope, dict(q=want((3, 4, 64), f32))),
+                     (_rope, dict(k=want((3, 2, 64), f32))), (_rope, dict(v=want((3, 2, 64), f32))),
+                     (_rope, dict(q_norm=want((64,), f32))), (_rope, dict(k_norm=want((64,), f32)))):
+        with pytest.raises(m27b.M27BError, match="no backward pass"):
+            call(torch, m27b, **kw)
+        with torch.no_grad(), pytest.raises(m27b.M27BError, match="current device"):
+            call(torch, m27b, **kw)
