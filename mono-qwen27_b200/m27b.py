@@ -958,7 +958,10 @@ def rope_table(n_pos, n_rot, theta, kind=ROPE_NONE, factor=1.0, original_ctx=0, 
     import torch
     if n_pos < 1 or n_rot < 2 or n_rot % 2:
         raise M27BError(f"rope_table: bad n_pos ({n_pos}) or n_rot ({n_rot})")
-    out = torch.empty(n_pos, n_rot // 2, 2, dtype=torch.float32, device=device)
+    # allocated on the stream that writes it: memory that work on another one is
+    # still to use is not handed out there
+    with torch.cuda.stream(stream):
+        out = torch.empty(n_pos, n_rot // 2, 2, dtype=torch.float32, device=device)
     s = _RopeScaling(kind, factor, original_ctx, beta_fast, beta_slow, attn_factor)
     err = ctypes.create_string_buffer(ERR_CAP)
     _check(_paged_lib().m27b_rope_table(_ptr(out), n_pos, n_rot, theta, ctypes.byref(s),

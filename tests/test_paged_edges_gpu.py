@@ -171,3 +171,17 @@ def test_many_small_weights_beside_a_large_one(torch, m27b, dtype, hd, n_seq, n_
     for b in range(0, n_seq, 13):
         _close(torch, out[b * n_tok:(b + 1) * n_tok], lse[b * n_tok:(b + 1) * n_tok], want, dtype)
     assert m27b.device_status() == 0
+
+
+def test_rope_table_on_another_stream_takes_no_memory_in_use(torch, m27b):
+    want = m27b.rope_table(20000, 128, 1e4)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(3):
+        old = torch.empty_like(want)
+        torch.cuda._sleep(20000000)
+        old.fill_(7.0)  # runs after the sleep
+        del old         # and its memory is free for this stream's next tensor
+        got = m27b.rope_table(20000, 128, 1e4, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
