@@ -21,9 +21,9 @@
  * synchronised or allocated, so every entry can be captured in a CUDA graph.
  * Lengths, tables and page ids are read on the device, so a captured graph
  * serves every state of the cache.  What only the device can see to be wrong
- * (a table row, page id or position out of range) is skipped and reported
- * through m27b_device_status (code 6): nothing outside the buffers is read or
- * written.
+ * (a table row, page id or position out of range) is reported through
+ * m27b_device_status (code 6): nothing outside the buffers is read or written,
+ * and each entry says what it does instead.
  */
 #ifndef M27B_PAGED_H
 #define M27B_PAGED_H
@@ -142,7 +142,12 @@ M27B_API size_t m27b_paged_attn_scratch_bytes(int n_q, int n_kv, int head_dim);
  * weights are rounded to the cache's type for their product with V.  Slots
  * that no row of the sequence sees may hold anything, infinities and NaN
  * included; a position that the sequence holds must be finite.  A row of q with
- * a NaN gets NaN in out and lse, and so does a row that sees one in K. */
+ * a NaN gets NaN in out and lse, and so does a row that sees one in K.
+ * scale is positive.
+ * Status 6: a page out of range that a row sees counts as keys and values of
+ * zero, a length beyond the table as the table's, a table row out of range as
+ * one without positions.  The rows of that sequence are then of no use; those of
+ * other sequences are right. */
 M27B_API bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const void *q, long long q_stride,
                               int n_q, float scale, int window, void *out, long long out_stride, float *lse,
                               void *scratch, cudaStream_t stream, char *err, size_t err_cap);

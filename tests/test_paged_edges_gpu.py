@@ -185,3 +185,37 @@ def test_rope_table_on_another_stream_takes_no_memory_in_use(torch, m27b):
         got = m27b.rope_table(20000, 128, 1e4, stream=s)
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("hd,q_lens,kv_lens", [(64, [1, 5, 1], [100, 90, 300]), (128, [150, 200, 90], [150, 300, 400])])
+def test_a_bad_page_counts_as_zeros_in_its_own_sequence(torch, m27b, hd, q_lens, kv_lens):
+    c = Cache(torch, m27b, kv_lens, 16, 2, hd, "bf16", 57)
+    q = torch.randn(sum(q_lens), 8, hd, device="cuda").bfloat16()
+    cu = _cu(torch, q_lens)
+    out, lse = _run(torch, m27b, c, q, cu)
+    k, v = _seq(torch, c, 1)
+    k[32:48] = v[32:48] = 0.0
+    mine = slice(q_lens[0], q_lens[0] + q_lens[1])
+    want = _attend(torch, q[mine], k, v, hd ** -0.5, 0)
+    for bad in (-1, c.k.shape[0], 1 << 30):
+        c.table[1, 2] = bad
+        got, got_l = _run(torch, m27b, c, q, cu)
+        assert m27b.device_status() == 6
+        _close(torch, got[mine], got_l[mine], want, "bf16")
+        for o in (slice(0, mine.start), slice(mine.stop, None)):
+            assert torch.equal(got[o], out[o]) and torch.equal(got_l[o], lse[o])
+    # a length beyond the table, and a row beyond it
+    c.table[1, 2] = int(c.tab[1, 2])
+    lens = c.lens.clone()
+    lens[1] = 1 << 30
+    got = torch.full_like(q, 7.0)
+    m27b.paged_attn(c.kv, q, cu, lens, got, m27b.paged_attn_scratch(8, 2, hd))
+    assert m27b.device_status() == 6
+    rows = torch.tensor([0, 3, 2], dtype=torch.int32, device="cuda")
+    none = torch.full_like(q, 7.0)
+    m27b.paged_attn(c.kv, q, cu, c.lens, none, m27b.paged_attn_scratch(8, 2, hd), rows=rows)
+    assert m27b.device_status() == 6 and bool((none[mine] == 0).all())
+    for b, o in ((0, slice(0, mine.start)), (2, slice(mine.stop, None))):  # the work is cut elsewhere: not bit for bit
+        want = _attend(torch, q[o], *_seq(torch, c, b), hd ** -0.5, 0)
+        _close(torch, got[o], None, want, "bf16")
+        _close(torch, none[o], None, want, "bf16")
