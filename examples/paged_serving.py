@@ -44,6 +44,7 @@ class Stack:
         cu = torch.zeros(len(rows) + 1, dtype=torch.int32, device="cuda")
         cu[1:] = lens_t.cumsum(0)
         self.pages.resize(rows_t, self.pages.lens[rows_t.long()] + lens_t)
+        self.pages.check()  # refused: lens are the old ones, and the append would overwrite the last positions
         q = torch.empty(len(x), self.n_q, self.hd, dtype=self.dtype, device="cuda")
         o = torch.empty_like(q)
         for kv, w_qkv, w_out in zip(self.kv, self.w_qkv, self.w_out):
@@ -58,6 +59,7 @@ class Stack:
     def fork(self, parent, children):
         i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
         self.pages.fork(i([parent] * len(children)), i(children))
+        self.pages.check()
 
     def free(self, rows):
         self.pages.free(torch.tensor(rows, dtype=torch.int32, device="cuda"))

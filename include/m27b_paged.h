@@ -186,7 +186,10 @@ M27B_API size_t m27b_pages_scratch_bytes(int n_pages, int n_rows, int n);
 /* Set the lengths of n rows to new_lens (device).  A row that grows takes the
  * lowest free pages, request by request; if its last page is half-filled and
  * shared, the row first gets a copy of its own (the next append writes
- * there).  A row that shrinks gives up its last pages. */
+ * there).  A row that shrinks gives up its last pages.  After a refused call the
+ * lengths are the old ones: an append of the new tokens would then overwrite the
+ * last positions, also in pages that other rows hold, so *status is to be read
+ * first. */
 M27B_API bool m27b_pages_resize(const M27BPages *pages, const M27BPagePool *pools, int n_pools, const int *rows,
                                 const int *new_lens, int n, void *scratch, int *status, cudaStream_t stream, char *err,
                                 size_t err_cap);

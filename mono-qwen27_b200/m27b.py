@@ -1050,7 +1050,9 @@ class PageSet:
     values) [n_planes, n_pages, ...] whose pages are contiguous; a plane is a
     layer's keys or values.  Requests are device int32 tensors.  A refused
     request (too few free pages, or a bad one) changes nothing and shows in
-    check()."""
+    check(); rope_append must not follow a refused resize, since the lengths are
+    still the old ones.  The set has one scratch and one status word: its calls
+    belong on one stream at a time."""
 
     def __init__(self, table, ref, lens, page_size, pool, max_requests=None):
         import torch
