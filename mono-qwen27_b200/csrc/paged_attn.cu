@@ -268,12 +268,12 @@ M27B_DI PaSeq pa_seq(const AttnArgs &a, int b, int tq, bool report) {
     const int2 t = seq_tokens(a.bt, b);
     s.q_lo = t.x, s.q_n = t.y - t.x;
     s.row = seq_row(a.bt, b, a.kv.n_rows);
-    const int cap = a.kv.n_cols * a.kv.page_size;
-    int len = s.row < 0 ? 0 : __ldg(a.bt.lens + s.row);
+    const int cap = a.kv.n_cols * a.kv.page_size, end = a.bt.cu_q[b + 1];
+    int len = s.row < 0 ? 0 : a.bt.lens[s.row];
     if (report && s.q_n > 0 && (s.row < 0 || len > cap)) paged_bad(a.status);
     len = max(0, min(len, cap));
     s.row = max(0, s.row);
-    s.base = (int)max((long long)-(1 << 30), (long long)len - __ldg(a.bt.cu_q + b + 1) + t.x);
+    s.base = (int)max((long long)-(1 << 30), (long long)len - end + t.x);
     s.nrt = (s.q_n + tq - 1) / tq;
     return s;
 }
@@ -490,7 +490,7 @@ struct PaShared {
 template <class Walk>
 M27B_DI int pa_page(const AttnArgs &a, const Walk &w, const int *ids, int p, int shift) {
     if (p >= a.kv.n_cols || (p << shift) >= w.sp.hi || (p + 1) << shift <= w.sp.lo) return a.kv.n_pages;
-    const int id = __ldg(ids + p);
+    const int id = ids[p];
     if (id >= 0 && id < a.kv.n_pages) return id;
     paged_bad(a.status);
     return a.kv.n_pages;
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 uint32_t v[16];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint4 z = live ? __ldg((const uint4 *)(qp + 32 * y) + e) : make_uint4(0, 0, 0, 0);
+                    const uint4 z = live ? *((const uint4 *)(qp + 32 * y) + e) : make_uint4(0, 0, 0, 0);
                     v[4 * e] = z.x, v[4 * e + 1] = z.y, v[4 * e + 2] = z.z, v[4 * e + 3] = z.w;
                 }
                 tmem_st16(lane_base + L::Q + half * (HD / 4) + 16 * y, v);

@@ -41,15 +41,20 @@ M27B_DI void paged_bad(int *status) {
     if (status) atomicCAS(status, 0, PAGED_BAD);
 }
 
+// Offsets, lengths, rows, tables and tokens may come from the launch before, whose
+// end pdl_wait() awaits while this kernel already runs: they are read by ordinary
+// loads, not by the read-only path (__ldg), which wants data that no one writes
+// during the kernel.
+
 // Rows [lo, hi) of sequence b in the token buffers, held to [0, n_tok).
 M27B_DI int2 seq_tokens(const M27BPagedBatch &bt, int b) {
-    const int lo = max(0, __ldg(bt.cu_q + b)), hi = min(bt.n_tok, __ldg(bt.cu_q + b + 1));
+    const int lo = max(0, bt.cu_q[b]), hi = min(bt.n_tok, bt.cu_q[b + 1]);
     return make_int2(lo, max(lo, hi));
 }
 
 // Table row of sequence b, -1 if it is out of range.
 M27B_DI int seq_row(const M27BPagedBatch &bt, int b, int n_rows) {
-    const int r = bt.rows ? __ldg(bt.rows + b) : b;
+    const int r = bt.rows ? bt.rows[b] : b;
     return r >= 0 && r < n_rows ? r : -1;
 }
 

@@ -36,7 +36,7 @@ M27B_DI int find_seq(const int *cu_q, int n, int t, int lane) {
     int lo = 0, hi = n;
     while (lo < hi) {
         const int step = (hi - lo + 31) / 32, i = lo + lane * step + step - 1;
-        const bool past = i < hi && __ldg(cu_q + i + 1) <= t;
+        const bool past = i < hi && cu_q[i + 1] <= t;
         lo += __popc(__ballot_sync(0xffffffffu, past)) * step;
         if (step == 1) break;
         hi = min(hi, lo + step - 1);
@@ -111,12 +111,12 @@ struct RopeToken {
     int rp;
 };
 M27B_DI bool rope_token(const RopeArgs &a, int t, int b, bool report, RopeToken &k) {
-    if (b >= a.bt.n_seq || t < __ldg(a.bt.cu_q + b)) return false;  // of no sequence
+    if (b >= a.bt.n_seq || t < a.bt.cu_q[b]) return false;  // of no sequence
     const int row = seq_row(a.bt, b, a.kv.n_rows);
-    const int p = row < 0 ? -1 : __ldg(a.bt.lens + row) - __ldg(a.bt.cu_q + b + 1) + t;
-    k.rp = a.rope.positions ? __ldg(a.rope.positions + t) : p;
+    const int p = row < 0 ? -1 : a.bt.lens[row] - a.bt.cu_q[b + 1] + t;
+    k.rp = a.rope.positions ? a.rope.positions[t] : p;
     const int pc = p / a.kv.page_size;
-    const int page = p >= 0 && pc < a.kv.n_cols ? __ldg(a.kv.table + (long long)row * a.kv.n_cols + pc) : -1;
+    const int page = p >= 0 && pc < a.kv.n_cols ? a.kv.table[(long long)row * a.kv.n_cols + pc] : -1;
     if (page < 0 || page >= a.kv.n_pages || k.rp < 0 || k.rp >= a.rope.n_pos) {
         if (report) paged_bad(a.status);
         return false;
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 2) k_rope_stream(const RopeArgs 
                     int lo = 0, hi = a.bt.n_seq;
                     while (lo < hi) {
                         const int mid = (lo + hi) / 2;
-                        if (__ldg(a.bt.cu_q + mid + 1) <= tl) lo = mid + 1;
+                        if (a.bt.cu_q[mid + 1] <= tl) lo = mid + 1;
                         else hi = mid;
                     }
                     if (!rope_token(a, tl, lo, true, k)) k.slot = -1;

@@ -219,3 +219,52 @@ def test_a_bad_page_counts_as_zeros_in_its_own_sequence(torch, m27b, hd, q_lens,
         want = _attend(torch, q[o], *_seq(torch, c, b), hd ** -0.5, 0)
         _close(torch, got[o], None, want, "bf16")
         _close(torch, none[o], None, want, "bf16")
+
+
+def test_steps_back_to_back_read_what_the_launch_before_wrote(torch, m27b):
+    # resize, append, attention of 70 rows, five steps in one graph, where each
+    # launch begins before the one before it has ended; and with a wait after each
+    ps, n_kv, hd, n_q, n = 16, 2, 128, 8, 70
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    rope, scr = m27b.rope_table(400, hd, 1e4), m27b.paged_attn_scratch(n_q, n_kv, hd)
+    rows, cu = i(list(range(n))), i(list(range(n + 1)))
+    x = torch.randn(5, n, n_q + 2 * n_kv, hd, device="cuda")
+    results = []
+    for graphed in (False, True):
+        pool = torch.zeros(2, 1000, ps, n_kv, hd, device="cuda").bfloat16()
+        pages = m27b.PageSet.empty(n, 20, 1000, ps, pool)
+        kv = m27b.PagedKV(pool[0], pool[1], pages.table)
+        start = i([(7 * r) % 150 for r in range(n)])
+        pages.resize(rows, start)
+        lens = [start + 1 + s for s in range(5)]
+        q, out = (torch.zeros(5, n, n_q, hd, device="cuda").bfloat16() for _ in range(2))
+        wait = (lambda: None) if graphed else torch.cuda.synchronize
+
+        def steps():
+            for s in range(5):
+                pages.resize(rows, lens[s])
+                wait()
+                m27b.rope_append(kv, x[s, :, :n_q], x[s, :, n_q:n_q + n_kv], x[s, :, n_q + n_kv:], cu, pages.lens, rope, q[s])
+                wait()
+                m27b.paged_attn(kv, q[s], cu, pages.lens, out[s], scr)
+                wait()
+
+        torch.cuda.synchronize()
+        if graphed:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                steps()
+            for _ in range(20):
+                pages.resize(rows, start)
+                pool.zero_()
+                out.zero_()
+                g.replay()
+                pages.check()
+                results.append((out.clone(), pages.lens.clone()))
+        else:
+            steps()
+            pages.check()
+            results.append((out.clone(), pages.lens.clone()))
+    for o, ln in results[1:]:
+        assert torch.equal(o, results[0][0]) and torch.equal(ln, results[0][1])
+    assert m27b.device_status() == 0
