@@ -958,7 +958,7 @@ template <int HD> struct PairShared {
     PaItem tail[PAIR_SOFTMAX];
     AttnArgs args;
     long long red[PAIR_THREADS / 32];
-    uint2 m[2][PA_ROWS];        // a row's m after a tile, by turns, with the tile's number + 1
+    uint64_t m[2][PA_ROWS];     // a row's m after a tile, by turns; above it the tile's number + 1
     float half[2][2][PA_ROWS];  // what the two warps of a row tell each other at an item's end
     uint32_t tmem;
     int abort;
@@ -992,20 +992,20 @@ M27B_DI float max3(float a, float b, float c) {
 }
 
 // The m that another warp stores with number `tag` (bounded, for a whole warp).
-M27B_DI bool pair_follow(const uint2 *p, uint32_t tag, float &m, volatile int *abort, int *status) {
-    uint2 v;
+M27B_DI bool pair_follow(const uint64_t *p, uint32_t tag, float &m, volatile int *abort, int *status) {
+    uint64_t v;
     const uint32_t at = smem_u32(p);
     uint32_t t0 = 0;
     bool here = true;
     for (unsigned it = 1;; ++it) {
-        asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-        if (v.y == tag) break;
+        asm volatile("ld.volatile.shared.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+        if ((uint32_t)(v >> 32) == tag) break;
         if ((it & 255u) == 0 && pa_give_up(t0, abort, status)) {
             here = false;
             break;
         }
     }
-    m = __uint_as_float(v.x);
+    m = __uint_as_float((uint32_t)v);
     return __all_sync(0xffffffffu, here) != 0;
 }
 
@@ -1066,7 +1066,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     }
     if (warp == PAIR_ISSUER) pair_tmem_alloc(&sh.tmem);
     if (tid == 0) sh.args = a;
-    if (tid < 2 * PA_ROWS) sh.m[tid >> 7][tid & 127].y = 0;
+    if (tid < 2 * PA_ROWS) sh.m[tid >> 7][tid & 127] = 0;
     pdl_wait();
     pdl_trigger();
     tc_fence_before();
@@ -1219,10 +1219,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         bool ok = true;
         if (lane == 0) sh.tail[warp] = PaItem{0, 0, 0, 0};
         // m after tile u of this quarter, from the warp that has the tile to the
-        // other: a word with its tile's number, so that no barrier is needed
+        // other: one 64-bit word with its tile's number (two words of a vector access
+        // have no order), so that no barrier is needed
         auto publish = [&](int u, float m) {
-            const uint2 v = make_uint2(__float_as_uint(m), (uint32_t)u + 1);
-            asm volatile("st.volatile.shared.v2.u32 [%0], {%1, %2};" ::"r"(smem_u32(&sh.m[u & 1][row])), "r"(v.x), "r"(v.y) : "memory");
+            const uint64_t v = (uint64_t)((uint32_t)u + 1) << 32 | __float_as_uint(m);
+            asm volatile("st.volatile.shared.u64 [%0], %1;" ::"r"(smem_u32(&sh.m[u & 1][row])), "l"(v) : "memory");
         };
         auto follow = [&](int u, float &m) { return pair_follow(&sh.m[u & 1][row], (uint32_t)u + 1, m, abort, a.status); };
         // arrivals that both CTAs' warps make in the first
