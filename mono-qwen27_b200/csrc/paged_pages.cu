@@ -20,7 +20,8 @@ constexpr unsigned COPY_CHUNK = COPY_THREADS * COPY_UNROLL * 16;  // bytes a CTA
 
 // Scratch: the header, then four int arrays.
 struct PagesHdr {
-    int go, n_moves, n_live, pad;
+    int go;       // fork, resize: the request stands
+    int n_moves;  // compact
 };
 struct PagesScratch {
     PagesHdr *hdr;
@@ -116,7 +117,6 @@ M27B_DI bool any_bad(bool bad) { return __syncthreads_or(bad) != 0; }
 M27B_DI void end_plan(const PagesArgs &a, int why) {
     if (threadIdx.x == 0) {
         a.s.hdr->go = !why;
-        a.s.hdr->n_moves = a.n;
         if (why && a.out) *a.out = why;
     }
 }
@@ -228,9 +228,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_compact_plan(const PagesArgs a
     __syncthreads();
     for (int k = threadIdx.x; k < movers; k += PLAN_THREADS) a.s.at[a.s.from[k]] = a.s.fresh[k];
     if (threadIdx.x == 0) {
-        a.s.hdr->go = 1;
         a.s.hdr->n_moves = movers;
-        a.s.hdr->n_live = live;
         if (a.out) *a.out = live;
     }
 }
@@ -417,7 +415,7 @@ bool check_pools(const M27BPagePool *p, int n, Pools *out, const char *what, cha
     return true;
 }
 
-// Enough CTAs that the reads in flight (two CTAs of 32 KB an SM) cover the memory's latency.
+// Four CTAs for each of the 148 SMs, each with up to 32 KB of reads in flight.
 unsigned copy_grid() { return 148 * 4; }
 
 bool requests(const void *a, const void *b, const void *scratch, int n, const char *what, char *err, size_t cap) {
