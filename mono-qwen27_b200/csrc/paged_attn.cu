@@ -30,9 +30,12 @@
 // What bounds it: decode (64 sequences of 300 to 8192 positions, 24 heads of
 // 256 over 4, 680 MB of cache) the memory: 120 us, 5.7 TB/s; a chunk of 4096
 // tokens over 8192 positions, same heads, the tensor pipe: 387 us with the pipe
-// busy 83 % of it at full clocks, 420 to 460 us (1.35 PFLOP/s) under the power
-// limit; few rows and short contexts the latency of the launch, the first loads
-// and the join: 13 us for one token over 769 positions.
+// busy 83 % of it at full clocks, 430 to 460 us back to back under the power
+// limit, 484 to 492 us a call from cold L2 (1.26 to 1.28 PFLOP/s); few rows and short contexts the latency of the launch, the first loads
+// and the join: 13 us for one token over 769 positions.  The same chunk with 16
+// heads of 128 over 8 (206 GFLOP, 224 us cold) and of 64 (255 us cold): the
+// hand-offs between the roles; the tensor pipe is busy 46 and 19 % of the time,
+// the exponentials' unit 49 and 41, the issue slots 36 and 38.
 //
 // A CTA's roles:
 //   * warp 8 streams the key tiles into a ring of slots, in the order in which
@@ -292,7 +295,8 @@ struct PaSpan {
 // behind: a decode batch of 64 sequences of 300 to 8192 positions ended after
 // 103 us on the median CTA and 146 us on the last.  Swept on that batch and
 // on a 4096-token chunk: 1, 2, 3, 4, 5, 6, 8 tiles 144, 133, 130, 122, 122, 123,
-// 126 us; pairs 4, 6, 8, 10, 12 tiles 430, 430, 434, 435, 468 us.
+// 126 us; pairs 4, 6, 8, 10, 12 tiles 430, 430, 434, 435, 468 us.  Both with
+// head_dim 256; 64 and 128 and items without tiles are charged the same, not swept.
 constexpr int PA_EXTRA = 4, PAIR_EXTRA = 6;
 template <int EX>
 M27B_DI int pa_units(const PaSpan &s) { return s.kt1 - s.kt0 + EX; }
@@ -1646,7 +1650,11 @@ bool m27b_paged_attn(const M27BPagedKV *kv, const M27BPagedBatch *batch, const v
     // 64 68 72 132; head_dim 128: 62 83 87 134 and 70 72 74 111; one sequence: 42 36
     // 38 36 and 36 38 40 38; a prompt of 4096 tokens over 8192 positions, 24 heads of
     // 256: 695 and 458, 16 heads of 128: 269 and 218.  (head_dim 64 has no pairs:
-    // a slot of 128 positions is 16 KB, and the shared memory keeps up.)
+    // the tensor pipe is busy a fifth of the time there, so that what a pair saves
+    // in shared memory is not what bounds it.)  The average is over the batch: 64
+    // single tokens over 2000 positions take 120 us, a chunk of 512 or 2048 tokens
+    // of another sequence 73 and 161, and both in one call 159 (single CTAs) and
+    // 294 (pairs), head_dim 256.
     const bool pair = (long long)batch->n_tok * G >= 192ll * batch->n_seq;
     bool maps = false;
     const cudaError_t e = kv->type == M27B_TYPE_BF16 ? pa_launch_hd<true>(a, G, pair, ctas, stream, &maps)

@@ -266,7 +266,9 @@ M27B_DI void norm_turn8(const RopeArgs &a, bool norms, bool norm, bool turn, con
 // which hold the kernel above to half of the bandwidth, are then off the warps'
 // path.  8192 tokens, from cold L2: 32 heads of 256 fp32 values 135 -> 74 us
 // (403 MB, 5.4 TB/s), 32 heads of 128 bf16 values 102 -> 43 us (134 MB, 3.1
-// TB/s: there the warps' instructions bound it).  A warp with whole heads, as
+// TB/s).  The same heads in fp32 take no longer (49 us against 48 a call): with
+// rows this short a unit's hand-offs bound it (1.6 us a unit and CTA), neither
+// the issue slots, 55 % busy, nor the memory.  A warp with whole heads, as
 // above, took 80 and 57 us; 12 and 16 warps 80 and 98 us, 47 and 68 us.
 constexpr int ROPE_WARPS = 8, ROPE_MAX_STAGES = 8;
 constexpr int ROPE_UNIT = 32 * 1024;
